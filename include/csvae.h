@@ -480,6 +480,73 @@ int cs_final_resample_static(const float* logw, const float* Zprops, int64_t TI,
                              int32_t Zd, const double* u, const cs_rng* rng, int64_t n, int64_t* idx, float* Zout,
                              void* stream);
 
+/* ---- beam search over chains (no counterpart in the reference; the deterministic sibling of the resampling) ------
+ * Element types of the entry points below. */
+#define CS_TYPE_F32 0
+#define CS_TYPE_BF16 1
+#define CS_TYPE_F16 2
+#define CS_TYPE_F64 3
+typedef struct {
+  int32_t B, K;          /* examples, beams per example (1 .. 2048) */
+  int64_t V;             /* values a beam can continue with */
+  int32_t W;             /* continuations to keep per example, 1 .. 64 */
+  int32_t logits_type;   /* CS_TYPE_F32 | CS_TYPE_BF16 | CS_TYPE_F16 */
+  int32_t scores_type;   /* CS_TYPE_F32 | CS_TYPE_F64, of `scores` and `out_scores` */
+  int32_t normalise;     /* 1: logits are turned into log-probabilities of their beam; 0: added as they are */
+  int64_t end_token;     /* the value a finished beam stays at (unused without `finished`) */
+  int64_t logits_stride[2];  /* elements between examples / beams of `logits` (values are adjacent) */
+  int64_t mask_stride[2];    /* bytes between examples / beams of `mask` (0: shared) */
+} cs_beam_cfg;
+/* Bytes of device memory cs_beam_select needs as `workspace` (8-byte aligned), or -1 for a bad configuration. */
+int64_t cs_beam_select_workspace(const cs_beam_cfg* cfg);
+/* Per example the W largest s[k,v] = logits[k,v] + (scores[k] - lse[k]), descending, ties to the lowest k*V + v, where
+ * lse[k] is the log of the sum of exponentials of beam k's allowed logits (0 with normalise = 0), all in 64 bits.
+ *   scores[B,K] (NULL: zeros), logits[B,K,V], mask (NULL: all) 1 = allowed: what is not allowed is neither a candidate
+ *   nor in the normaliser, whatever its logit holds; finished[B,K] (NULL: none): such a beam has one candidate,
+ *   end_token with its score unchanged, and its logits are not read.
+ * NaN and -inf are no candidates; a beam whose normaliser is not finite (a NaN or +inf among its allowed logits) has
+ * none.  out_scores[B,W], parents[B,W], tokens[B,W] (int64); where there are fewer than W candidates: -inf, the
+ * slot's own index (at most K-1), -1.  Candidates of one beam that 64 bits do not tell apart keep their logits' order.
+ * Two launches; the result does not depend on anything but the arguments. */
+int cs_beam_select(const cs_beam_cfg* cfg, const void* scores, const void* logits, const uint8_t* mask,
+                   const uint8_t* finished, void* out_scores, int64_t* parents, int64_t* tokens, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+/* dst[o,b,w,:] = src[o,b,parents[b,w],:] for o < outer, b < B, w < W; rows of row_bytes adjacent bytes, the strides of
+ * (outer, example, chain) in bytes.  A parent outside [0,K) leaves its row of dst as it was.  In place with
+ * src == dst: W == K <= 64 and equal strides; otherwise the memory from the first to the last byte of either must not
+ * overlap.  Rows of dst must not overlap each other. */
+int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_t B, int32_t K, int32_t W, int64_t row_bytes,
+                    const int64_t src_stride[3], const int64_t dst_stride[3], const int64_t* parents, void* stream);
+
+/* ---- history ring in 8 or 4 bits (no counterpart in the reference, whose queues are float32 or bool) ---------------
+ * data: [T,B,K] records of cs_qcache_record_bytes each (16-byte aligned); a record holds the codes of D values, then the
+ * scales of its groups of `group` consecutive values.
+ *   CS_QFMT_INT8   groups of 32, 64 or 128; scale s = max(float32(largest finite magnitude / 127), 2^-126); code = the
+ *                  integer nearest to x / s, ties to even; -128 where x is not finite (reads as NaN)
+ *   CS_QFMT_MXFP8  OCP Microscaling e4m3, groups of 32, scale 2^e with the smallest e >= -127 that clips nothing; nearest,
+ *                  ties to even; not finite: NaN
+ *   CS_QFMT_MXFP4  the same with e2m1; a group with a value that is not finite reads as NaN */
+#define CS_QFMT_INT8 0
+#define CS_QFMT_MXFP8 1
+#define CS_QFMT_MXFP4 2
+typedef struct {
+  void* data;
+  int64_t T, B;
+  int32_t K, D, fmt, group;
+} cs_qcache;
+int64_t cs_qcache_record_bytes(int32_t fmt, int32_t group, int32_t D);   /* -1: bad arguments */
+/* Quantises X[n,B,K,D] (n <= T; D values adjacent, the strides of (step, example, chain) in elements) into the slots
+ * (start + i) mod T, i < n.  start[B,K] (NULL: start0 for all; negative: nothing of that chain is written),
+ * count[B,K] (NULL: n): only the first count states of a chain are read and written; every other record stays as it
+ * is. */
+int cs_qcache_write(const cs_qcache* c, const void* X, int32_t x_type, int64_t n, const int64_t x_stride[3],
+                    const int64_t* start, int64_t start0, const int64_t* count, void* stream);
+/* out[i,b,j,:] = the state at slot slots[i,b,j] (NULL: (start0 + i) mod T) of chain chains[i,b,j] (NULL: j, and J must
+ * be K) of example b; zeros where slot or chain do not exist.  slots / chains: int64 [N,B,J]; out_stride of
+ * (i, example, j) in elements. */
+int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t start0, const int64_t* chains, int64_t N, int32_t J,
+                   void* out, int32_t out_type, const int64_t out_stride[3], void* stream);
+
 /* Draws the built-in RNG would use, written out for tests: standard normals / uniforms of
  * `stream_id` (CS_STREAM_* in csrc/cs_common.h) for rows example_offset + [0,rows) and
  * elements [0,cols). */

@@ -1,0 +1,129 @@
+"""CPU: arguments that the beam operators and the quantised history refuse, in the wrappers and at the C entries (no
+entry gets as far as a launch)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from vae_conditional_sampling_amd import _lib
+from vae_conditional_sampling_amd.sampling import beam
+from vae_conditional_sampling_amd.sampling.utils import QuantisedHistory
+
+EINVAL = -1
+
+
+def cfg(B=2, K=3, V=10, W=4, logits=0, scores=0, end=0):
+    return _lib.cs_beam_cfg(B, K, V, W, logits, scores, 1, end)
+
+
+@pytest.mark.parametrize("bad", [dict(W=0), dict(W=65), dict(K=0), dict(K=2049), dict(V=0), dict(V=1 << 31), dict(B=-1),
+                                 dict(logits=3), dict(logits=7), dict(scores=1), dict(B=2 ** 30, K=2048, V=10 ** 9)])
+def test_bad_configurations_have_no_workspace_and_are_refused(bad):
+    L = _lib.lib()
+    c = cfg(**bad)
+    assert L.cs_beam_select_workspace(C.byref(c)) == -1
+    p = 4096   # never used
+    assert L.cs_beam_select(C.byref(c), p, p, None, None, p, p, p, p, 1 << 40, None) == EINVAL
+
+
+def test_select_refuses_missing_buffers_a_small_workspace_and_an_end_token_outside():
+    L = _lib.lib()
+    c = cfg()
+    need = L.cs_beam_select_workspace(C.byref(c))
+    assert need > 0 and L.cs_beam_select_workspace(C.byref(cfg(B=0))) == 0
+    p = 4096
+    for hole in range(5):
+        a = [p] * 5
+        a[hole] = None
+        assert L.cs_beam_select(C.byref(c), p, a[0], None, None, a[1], a[2], a[3], a[4], need, None) == EINVAL
+    assert L.cs_beam_select(C.byref(c), p, p, None, None, p, p, p, p, need - 1, None) == EINVAL
+    assert L.cs_beam_select(C.byref(c), p, p, None, None, p, p, p, p + 4, need, None) == EINVAL
+    for end in (-1, 10):
+        assert L.cs_beam_select(C.byref(cfg(end=end)), p, p, None, p, p, p, p, p, need, None) == EINVAL
+    assert L.cs_beam_select(C.byref(cfg(B=0)), None, None, None, None, None, None, None, None, 0, None) == 0
+    assert L.cs_beam_select(None, p, p, None, None, p, p, p, p, need, None) == EINVAL
+    assert L.cs_beam_select_workspace(None) == -1
+
+
+def test_reorder_refuses_overlaps():
+    L = _lib.lib()
+    s = lambda *v: (C.c_int64 * 3)(*v)
+    call = lambda src, dst, outer, B, K, W, row, ss, ds: L.cs_beam_reorder(src, dst, outer, B, K, W, row, ss, ds, 4096, None)
+    base = 1 << 20
+    lay = s(2 * 3 * 8, 3 * 8, 8)
+    assert call(base, base, 4, 2, 3, 2, 8, lay, lay) == EINVAL                    # in place with another number of chains
+    assert call(base, base, 4, 2, 65, 65, 8, s(2 * 65 * 8, 65 * 8, 8), s(2 * 65 * 8, 65 * 8, 8)) == EINVAL
+    assert call(base, base, 4, 2, 3, 3, 8, lay, s(2 * 3 * 16, 3 * 16, 16)) == EINVAL
+    assert call(base, base + 8, 4, 2, 3, 3, 8, lay, lay) == EINVAL                # shifted onto itself
+    assert call(base, base + 1000, 4, 2, 3, 3, 8, lay, s(0, 3 * 8, 8)) == EINVAL    # rows of the destination on each other
+    assert call(base, base + 1000, 4, 2, 3, 3, 8, lay, s(48, 16, 8)) == EINVAL      # the third chain lies in the next example
+    assert call(base, base + 1000, 4, 2, 3, 3, 8, s(-48, 24, 8), lay) == EINVAL
+    assert call(None, base, 4, 2, 3, 3, 8, lay, lay) == EINVAL
+    assert call(base, base, 4, 2, 0, 3, 8, lay, lay) == EINVAL
+    assert call(None, None, 0, 2, 3, 3, 8, lay, lay) == 0
+    assert call(None, None, 4, 2, 3, 3, 0, lay, lay) == 0
+
+
+def test_ring_refusals():
+    L = _lib.lib()
+    for fmt, group, D in ((0, 16, 8), (0, 256, 8), (1, 64, 8), (2, 128, 8), (3, 32, 8), (-1, 32, 8), (0, 32, 0), (0, 32, 1 << 25)):
+        assert L.cs_qcache_record_bytes(fmt, group, D) == -1
+    assert L.cs_qcache_record_bytes(0, 64, 43) == 48      # 43 codes (44) and a scale
+    assert L.cs_qcache_record_bytes(0, 32, 43) == 64
+    assert L.cs_qcache_record_bytes(1, 32, 43) == 48
+    assert L.cs_qcache_record_bytes(2, 32, 43) == 32
+    assert L.cs_qcache_record_bytes(2, 32, 1) == 16
+    s = (C.c_int64 * 3)(6, 3, 1)
+    c = _lib.cs_qcache(4096, 5, 2, 3, 7, 0, 64)
+    w = lambda c, X=4096, type=0, n=1, start=None, start0=0: L.cs_qcache_write(C.byref(c), X, type, n, s, start, start0, None, None)
+    assert w(c, n=6) == EINVAL and w(c, n=-1) == EINVAL           # more states than slots
+    assert w(c, start0=-1) == EINVAL and w(c, X=None) == EINVAL and w(c, type=3) == EINVAL
+    assert w(c, n=0, X=None) == 0
+    assert w(_lib.cs_qcache(4097, 5, 2, 3, 7, 0, 64)) == EINVAL    # alignment of the ring
+    assert w(_lib.cs_qcache(None, 5, 2, 3, 7, 0, 64)) == EINVAL
+    assert w(_lib.cs_qcache(4096, 0, 2, 3, 7, 0, 64)) == EINVAL
+    r = lambda c, slots=None, start0=0, chains=None, N=1, J=3, out=4096, type=0: L.cs_qcache_read(
+        C.byref(c), slots, start0, chains, N, J, out, type, s, None)
+    assert r(c, J=2) == EINVAL                                    # fewer rows than chains, and no chains named
+    assert r(c, start0=-1) == EINVAL and r(c, out=None) == EINVAL and r(c, type=3) == EINVAL and r(c, N=-1) == EINVAL
+    assert r(c, N=0, out=None) == 0
+    assert r(_lib.cs_qcache(4096, 5, 2, 3, 7, 1, 64)) == EINVAL
+
+
+def test_wrappers_refuse_cpu_tensors_shapes_and_types():
+    x = torch.zeros(2, 3, 10)
+    with pytest.raises(_lib.CsError, match="no CPU path"):
+        beam.beam_select(None, x, 2)
+    with pytest.raises(_lib.CsError, match=r"\[B,K,V\]"):
+        beam.beam_select(None, x[0], 2)
+    p = torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(_lib.CsError, match="no CPU path"):
+        beam.reorder_states(x, p)
+    with pytest.raises(_lib.CsError, match="parents"):
+        beam.reorder_states(x, p.int())
+    with pytest.raises(_lib.CsError, match="parents"):
+        beam.reorder_states(x, p[:1])
+    with pytest.raises(_lib.CsError, match="out must be"):
+        beam.reorder_states(x, p, out=torch.zeros(2, 4, 10))
+    with pytest.raises(_lib.CsError, match="axis"):
+        beam.reorder_states(x, p, batch_dim=2)
+    with pytest.raises(NotImplementedError):
+        QuantisedHistory(4, (2, 3, 7), "int4", device="cpu")
+    with pytest.raises(_lib.CsError):
+        QuantisedHistory(4, (2, 3, 7), "mxfp8", group=64, device="cpu")
+    with pytest.raises(_lib.CsError):
+        QuantisedHistory(0, (2, 3, 7), "int8", device="cpu")
+    q = QuantisedHistory(4, (2, 3, 7), "int8", device="cpu")
+    for call in (lambda: q.write(torch.zeros(2, 3, 7), 0), lambda: q.read(p), lambda: q.read_steps(0, 1), lambda: q.reorder(p)):
+        with pytest.raises(_lib.CsError, match="no CPU path"):
+            call()
+    with pytest.raises(_lib.CsError, match="states must be"):
+        q.write(torch.zeros(2, 3, 8), 0)
+    with pytest.raises(_lib.CsError, match="states must be"):
+        q.write(torch.zeros(2, 3, 7, dtype=torch.float64), 0)
+    with pytest.raises(_lib.CsError, match="slots"):
+        q.read(p[:, :2])
+    with pytest.raises(_lib.CsError, match="slots"):
+        q.read(p.int())
+    with pytest.raises(_lib.CsError, match="out must be"):
+        q.read(p, out=torch.zeros(2, 3, 8))

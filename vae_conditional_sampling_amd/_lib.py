@@ -158,6 +158,21 @@ def make_acmwg_bufs(**tensors):
     return b
 
 
+class cs_beam_cfg(C.Structure):
+    _fields_ = [("B", C.c_int32), ("K", C.c_int32), ("V", C.c_int64), ("W", C.c_int32), ("logits_type", C.c_int32),
+                ("scores_type", C.c_int32), ("normalise", C.c_int32), ("end_token", C.c_int64),
+                ("logits_stride", C.c_int64 * 2), ("mask_stride", C.c_int64 * 2)]
+
+
+class cs_qcache(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("T", C.c_int64), ("B", C.c_int64), ("K", C.c_int32), ("D", C.c_int32),
+                ("fmt", C.c_int32), ("group", C.c_int32)]
+
+
+# element types and formats of the beam / quantised-history entry points
+CS_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
+CS_QFMT = {"int8": 0, "mxfp8": 1, "mxfp4": 2}
+
 _lib = None
 
 
@@ -225,6 +240,14 @@ def lib():
     L.cs_latent_wasserstein.argtypes = [vp, vp, i64, i32, i32, vp, vp]
     L.cs_sample_impute.argtypes = [vp, i32, vp, C.POINTER(cs_rng), u32, vp, vp, i64, i32, i32, vp, vp, i32, vp]
     L.cs_sample_impute2.argtypes = [vp, i32, vp, vp, C.POINTER(cs_rng), u32, vp, vp, i64, i32, i32, vp, vp, i32, vp]
+    L.cs_beam_select_workspace.restype = i64
+    L.cs_beam_select_workspace.argtypes = [C.POINTER(cs_beam_cfg)]
+    L.cs_beam_select.argtypes = [C.POINTER(cs_beam_cfg), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.cs_beam_reorder.argtypes = [vp, vp, i64, i64, i32, i32, i64, C.POINTER(i64), C.POINTER(i64), vp, vp]
+    L.cs_qcache_record_bytes.restype = i64
+    L.cs_qcache_record_bytes.argtypes = [i32, i32, i32]
+    L.cs_qcache_write.argtypes = [C.POINTER(cs_qcache), vp, i32, i64, C.POINTER(i64), vp, i64, vp, vp]
+    L.cs_qcache_read.argtypes = [C.POINTER(cs_qcache), vp, i64, vp, i64, i32, vp, i32, C.POINTER(i64), vp]
     for fn in ("cs_rng_normal", "cs_rng_uniform", "cs_rng_uniform64"):
         getattr(L, fn).argtypes = [C.POINTER(cs_rng), u32, i64, i32, vp, vp]
     _lib = L
@@ -266,6 +289,31 @@ def ptr(t):
     if not t.is_contiguous():
         raise CsError("tensor must be contiguous")
     return t.data_ptr()
+
+
+def on_device(*tensors):
+    """The CUDA device of all given tensors (None is passed over), for entry points that also serve tensors of another
+    device than the current one."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise CsError("libcsvae operates on device tensors only (no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise CsError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def call_on(dev, fn, *args):
+    """``check(fn(*args, stream))`` on the current stream of ``dev``, with ``dev`` current for the call."""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
 
 
 def make_rng(seed, iteration=0, example_offset=0):

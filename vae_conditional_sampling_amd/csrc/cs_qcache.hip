@@ -1,0 +1,304 @@
+// History ring in 8 or 4 bits: past states [T,B,K,D] quantised as they are written and read back by slot and chain.  The
+// counterpart of the float32 and uint8 rings (cs_history_enqueue, cs_history_concat) for real-valued data.
+//
+// A state is one record: its codes, then the scales of its groups (consecutive values along D), padded to 16 bytes.
+// Codes and scales lie together because states are fetched singly, by a slot per chain: a MiniBooNE state (D = 43) in 8
+// bits is one record of 48 bytes instead of a row of 172 and is fetched with one or two cache lines.
+//   int8   scale s = max(fl32(largest finite magnitude / 127), 2^-126), code = the integer nearest to the real quotient
+//          x / s, ties to even; -128 marks a value that was not finite (it reads as NaN).
+//   mxfp8  e4m3 elements, mxfp4 e2m1 elements of OCP Microscaling: scale 2^e as an e + 127 byte, groups of 32.  e is the
+//          smallest with the largest finite magnitude within the elements' range, so that no value is clipped and every
+//          rounding is off by at most half a step.  Not finite: the NaN of e4m3; e2m1 has none, there the group's
+//          scale becomes 255 and the group reads as NaN.
+// A lane holds 8 values, G / 8 neighbouring lanes share a group's maximum; both directions are bound by memory.
+#include "cs_common.h"
+
+namespace {
+
+constexpr int QC_LANE = 8;     // values a lane holds
+
+struct QcArgs {
+  cs_qcache c;
+  int64_t record;              // bytes
+  int32_t code_bytes;          // of a record, rounded up to 4
+  int32_t lanes;               // lanes of a row: groups * G / 8
+  int32_t rows_per_block;
+  int64_t rows, chains;        // rows of the call; B * K (write) or B * J (read)
+  int32_t J;
+  const void* x;               // write
+  void* out;                   // read
+  int64_t stride[3];
+  int64_t start0;
+  const int64_t *start, *count, *slots, *from;
+};
+
+struct QcBf16 { uint16_t u; };
+__device__ __forceinline__ float qc_float(float v) { return v; }
+__device__ __forceinline__ float qc_float(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float qc_float(QcBf16 v) { return __uint_as_float((uint32_t)v.u << 16); }
+__device__ __forceinline__ void qc_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void qc_store(_Float16* p, float v) { *p = (_Float16)v; }
+__device__ __forceinline__ void qc_store(QcBf16* p, float v) {   // nearest, ties to even
+  const uint32_t u = __float_as_uint(v);
+  p->u = (uint16_t)(v != v ? 0x7fc0u : (u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+
+// Codes of 8 values of a group whose largest finite magnitude is `top`; `fine`: all of the GROUP's values are finite.
+// The scale goes to `scale` (int8: a float's bits, else the byte).
+template <int FMT>
+__device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, uint32_t* codes, uint32_t* scale) {
+  if (FMT == CS_QFMT_INT8) {
+    const float s = fmaxf(top / 127.0f, 1.17549435e-38f);
+    const float inv = 1.0f / s;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < QC_LANE; ++i) {
+      // x * inv is off by less than one, the remainder x - q s is exact (a multiple of the last place of s or x below
+      // 2^24 of them), so one correction gives the nearest integer of the real quotient
+      const float v = __builtin_fabsf(x[i]) <= 3.402823466e+38f ? x[i] : 0.0f;
+      float q = __builtin_rintf(v * inv);
+      const float r = 2.0f * __builtin_fmaf(-q, s, v);
+      const float away = __builtin_fabsf(r);
+      const bool odd = ((int)q & 1) != 0;
+      if (away > s || (away == s && odd)) q += r > 0.0f ? 1.0f : -1.0f;
+      q = fminf(fmaxf(q, -127.0f), 127.0f);
+      const uint32_t c = v == x[i] ? (uint32_t)(int)q & 0xffu : 0x80u;
+      w[i >> 2] |= c << (8 * (i & 3));
+    }
+    codes[0] = w[0]; codes[1] = w[1];
+    *scale = __float_as_uint(s);
+    return;
+  }
+  const float largest = FMT == CS_QFMT_MXFP8 ? 0.875f : 0.75f;       // 448 = 0.875 * 2^9, 6 = 0.75 * 2^3
+  int e = -127;
+  if (top > 0.0f) {
+    e = __builtin_amdgcn_frexp_expf(top) - (FMT == CS_QFMT_MXFP8 ? 9 : 3) + (__builtin_amdgcn_frexp_mantf(top) > largest ? 1 : 0);
+    e = e < -127 ? -127 : e;
+  }
+  float y[QC_LANE];
+#pragma unroll
+  for (int i = 0; i < QC_LANE; ++i) {
+    const bool ok = __builtin_fabsf(x[i]) <= 3.402823466e+38f;
+    y[i] = ok ? __builtin_amdgcn_ldexpf(x[i], -e) : (FMT == CS_QFMT_MXFP8 ? __builtin_nanf("") : 0.0f);
+  }
+  if (FMT == CS_QFMT_MXFP8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
+      codes[h] = (uint32_t)w;
+    }
+  } else {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
+    codes[0] = w;
+  }
+  *scale = FMT == CS_QFMT_MXFP4 && !fine ? 255u : (uint32_t)(e + 127);
+}
+
+template <int FMT>
+__device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale, float* v) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if (FMT == CS_QFMT_INT8) {
+    const float s = __uint_as_float(scale);
+#pragma unroll
+    for (int i = 0; i < QC_LANE; ++i) {
+      const int q = (int8_t)(codes[i >> 2] >> (8 * (i & 3)));
+      // (the scale of the very largest float32 values is rounded up: their product is kept finite)
+      const float p = fminf(fmaxf((float)q * s, -3.402823466e+38f), 3.402823466e+38f);
+      v[i] = q == -128 ? __builtin_nanf("") : p;
+    }
+    return;
+  }
+  const int e = (int)scale - 127;
+  if (FMT == CS_QFMT_MXFP8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[h], true);
+      v[4 * h] = a.x; v[4 * h + 1] = a.y; v[4 * h + 2] = b.x; v[4 * h + 3] = b.y;
+    }
+  } else {
+    const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 1),
+             c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 3);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+  }
+#pragma unroll
+  for (int i = 0; i < QC_LANE; ++i) v[i] = scale == 255u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v[i], e);
+}
+
+// the slot of row r of a call (n steps of `chains` chains from `start` on); -1: not in the call
+__device__ __forceinline__ int64_t qc_slot(const QcArgs& a, int64_t i, int64_t chain) {
+  if (a.count && i >= a.count[chain]) return -1;
+  const int64_t s = a.start ? a.start[chain] : a.start0;
+  if (s < 0) return -1;
+  return (s % a.c.T + i) % a.c.T;
+}
+
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
+  const int ry = threadIdx.x / a.lanes;
+  const int64_t row = (int64_t)blockIdx.x * a.rows_per_block + ry;
+  const bool live = ry < a.rows_per_block && row < a.rows;
+  const int64_t i = live ? row / a.chains : 0, chain = live ? row - i * a.chains : 0;
+  const int64_t slot = live ? qc_slot(a, i, chain) : -1;
+  const int64_t b = chain / a.c.K, k = chain - b * a.c.K;
+  const T* x = (const T*)a.x + i * a.stride[0] + b * a.stride[1] + k * a.stride[2];
+  char* rec = (char*)a.c.data + ((slot < 0 ? 0 : slot) * a.chains + chain) * a.record;
+  const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
+  // (lanes of a row: a multiple of the lanes of a group, which divide 64; whole groups of lanes take part or none)
+  for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
+    const int d0 = l * QC_LANE;
+    float v[QC_LANE];
+    float top = 0.0f;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < QC_LANE; ++e) v[e] = slot >= 0 && d0 + e < D ? qc_float(x[d0 + e]) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < QC_LANE; ++e) {
+      const float m = __builtin_fabsf(v[e]);
+      const bool ok = m <= 3.402823466e+38f;
+      top = fmaxf(top, ok ? m : 0.0f);
+      fine = fine && ok;
+    }
+    int bad = fine ? 0 : 1;
+    for (int o = 1; o < lg; o <<= 1) {
+      top = fmaxf(top, __shfl_xor(top, o));
+      bad |= __shfl_xor(bad, o);
+    }
+    uint32_t codes[2] = {0, 0}, scale = 0;
+    qc_encode<FMT>(v, top, bad == 0, codes, &scale);
+    if (slot >= 0) {
+      const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
+      if (c0 < a.code_bytes) *(uint32_t*)(rec + c0) = codes[0];
+      if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) *(uint32_t*)(rec + c0 + 4) = codes[1];
+      if (l % lg == 0) {
+        if (FMT == CS_QFMT_INT8) *(uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) = scale;
+        else *(uint8_t*)(rec + a.code_bytes + l / lg) = (uint8_t)scale;
+      }
+    }
+  }
+}
+
+template <int FMT, typename T>
+__global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
+  const int ry = threadIdx.x / a.lanes;
+  const int64_t row = (int64_t)blockIdx.x * a.rows_per_block + ry;
+  if (ry >= a.rows_per_block || row >= a.rows) return;
+  const int64_t i = row / a.chains, chain = row - i * a.chains;
+  const int64_t b = chain / a.J, j = chain - b * a.J;
+  const int64_t slot = a.slots ? a.slots[row] : qc_slot(a, i, chain);
+  const int64_t k = a.from ? a.from[row] : j;
+  const bool there = slot >= 0 && slot < a.c.T && k >= 0 && k < a.c.K;
+  const char* rec = (const char*)a.c.data + (there ? ((slot * a.c.B + b) * a.c.K + k) * a.record : 0);
+  T* out = (T*)a.out + i * a.stride[0] + b * a.stride[1] + j * a.stride[2];
+  const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
+  for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
+    const int d0 = l * QC_LANE;
+    if (d0 >= D) break;
+    uint32_t codes[2] = {0, 0}, scale = 127;
+    if (there) {
+      const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
+      codes[0] = *(const uint32_t*)(rec + c0);
+      if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) codes[1] = *(const uint32_t*)(rec + c0 + 4);
+      scale = FMT == CS_QFMT_INT8 ? *(const uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) : *(const uint8_t*)(rec + a.code_bytes + l / lg);
+    }
+    float v[QC_LANE];
+    qc_decode<FMT>(codes, scale, v);
+#pragma unroll
+    for (int e = 0; e < QC_LANE; ++e)
+      if (d0 + e < D) qc_store(out + d0 + e, v[e]);
+  }
+}
+
+int64_t code_bytes_of(int fmt, int64_t D) {
+  const int64_t n = fmt == CS_QFMT_MXFP4 ? (D + 1) / 2 : D;
+  return (n + 3) / 4 * 4;
+}
+
+int check_qcache(const cs_qcache* c) {
+  CS_REQUIRE(c, "null argument");
+  CS_REQUIRE(c->T >= 1 && c->B >= 0 && c->K >= 1 && c->D >= 1, "bad sizes");
+  CS_REQUIRE(c->fmt == CS_QFMT_INT8 || c->fmt == CS_QFMT_MXFP8 || c->fmt == CS_QFMT_MXFP4, "unknown format");
+  if (c->fmt == CS_QFMT_INT8) CS_REQUIRE(c->group == 32 || c->group == 64 || c->group == 128, "int8: groups of 32, 64 or 128");
+  else CS_REQUIRE(c->group == 32, "mxfp8 / mxfp4: groups of 32");
+  CS_REQUIRE(c->D <= (1 << 24), "rows too long");
+  return CS_OK;
+}
+
+template <bool WRITE, int FMT>
+void launch_type(const QcArgs& a, int type, dim3 grid, hipStream_t st) {
+  if (WRITE) {
+    if (type == CS_TYPE_F32) hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, float>), grid, dim3(256), 0, st, a);
+    else if (type == CS_TYPE_BF16) hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, QcBf16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, _Float16>), grid, dim3(256), 0, st, a);
+  } else {
+    if (type == CS_TYPE_F32) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, float>), grid, dim3(256), 0, st, a);
+    else if (type == CS_TYPE_BF16) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, QcBf16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, _Float16>), grid, dim3(256), 0, st, a);
+  }
+}
+
+template <bool WRITE>
+int launch(QcArgs& a, int type, hipStream_t st) {
+  const cs_qcache& c = a.c;
+  CS_REQUIRE(type == CS_TYPE_F32 || type == CS_TYPE_BF16 || type == CS_TYPE_F16, "states are float32, bfloat16 or float16");
+  CS_REQUIRE(((uintptr_t)c.data & 15) == 0, "the ring must be 16-byte aligned");
+  a.record = cs_qcache_record_bytes(c.fmt, c.group, c.D);
+  a.code_bytes = (int32_t)code_bytes_of(c.fmt, c.D);
+  a.lanes = (c.D + c.group - 1) / c.group * (c.group / QC_LANE);
+  a.rows_per_block = a.lanes >= 256 ? 1 : 256 / a.lanes;
+  const int64_t blocks = (a.rows + a.rows_per_block - 1) / a.rows_per_block;
+  CS_REQUIRE(blocks <= INT32_MAX, "too many states for one call");
+  const dim3 grid((unsigned)blocks);
+  if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, grid, st);
+  else if (c.fmt == CS_QFMT_MXFP8) launch_type<WRITE, CS_QFMT_MXFP8>(a, type, grid, st);
+  else launch_type<WRITE, CS_QFMT_MXFP4>(a, type, grid, st);
+  CS_HIP(hipGetLastError());
+  return CS_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t cs_qcache_record_bytes(int32_t fmt, int32_t group, int32_t D) {
+  const cs_qcache c = {nullptr, 1, 1, 1, D, fmt, group};
+  if (check_qcache(&c)) return -1;
+  const int64_t groups = (D + group - 1) / group;
+  return (code_bytes_of(fmt, D) + groups * (fmt == CS_QFMT_INT8 ? 4 : 1) + 15) / 16 * 16;
+}
+
+extern "C" int cs_qcache_write(const cs_qcache* c, const void* X, int32_t x_type, int64_t n, const int64_t x_stride[3],
+                               const int64_t* start, int64_t start0, const int64_t* count, void* stream) {
+  if (int rc = check_qcache(c)) return rc;
+  CS_REQUIRE(n >= 0 && n <= c->T, "at most T states of a chain per call");
+  CS_REQUIRE(start || start0 >= 0, "negative start");
+  if (n == 0 || c->B == 0) return CS_OK;
+  CS_REQUIRE(c->data && X && x_stride, "null argument");
+  QcArgs a = {};
+  a.c = *c;
+  a.chains = c->B * c->K;
+  a.rows = n * a.chains;
+  a.x = X; a.start = start; a.start0 = start0; a.count = count;
+  for (int i = 0; i < 3; ++i) a.stride[i] = x_stride[i];
+  return launch<true>(a, x_type, (hipStream_t)stream);
+}
+
+extern "C" int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t start0, const int64_t* chains, int64_t N, int32_t J,
+                              void* out, int32_t out_type, const int64_t out_stride[3], void* stream) {
+  if (int rc = check_qcache(c)) return rc;
+  CS_REQUIRE(N >= 0 && J >= 1, "bad sizes");
+  CS_REQUIRE(chains || J == c->K, "without chains a row is read of every chain");
+  CS_REQUIRE(slots || start0 >= 0, "negative start");
+  if (N == 0 || c->B == 0) return CS_OK;
+  CS_REQUIRE(c->data && out && out_stride, "null argument");
+  QcArgs a = {};
+  a.c = *c;
+  a.chains = c->B * J;
+  a.rows = N * a.chains;
+  a.J = J;
+  a.out = out; a.slots = slots; a.start0 = start0; a.from = chains;
+  for (int i = 0; i < 3; ++i) a.stride[i] = out_stride[i];
+  return launch<false>(a, out_type, (hipStream_t)stream);
+}

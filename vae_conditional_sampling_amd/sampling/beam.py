@@ -1,0 +1,153 @@
+"""Beam search over chains: the deterministic sibling of the multinomial / systematic resampling.
+
+The beams of an example are its chains ``[B,K]``; every beam can continue with ``V`` values (proposals, categories, tokens).
+``beam_select`` keeps the ``width`` best continuations of an example, ``reorder_states`` lets what is kept per chain (latents
+``[B,K,Zd]``, a history ``[T,B,K,D]``, drawn values) follow the chosen parents.  ``sampling.utils.QuantisedHistory`` keeps a
+history in 8 or 4 bits and reorders it likewise.  The reference has no counterpart.
+"""
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _lib
+
+MAX_WIDTH = 64
+
+
+class BeamStep(NamedTuple):
+    scores: torch.Tensor    # [B,W], the type of the given scores
+    parents: torch.Tensor   # [B,W] int64: the beam that is continued
+    tokens: torch.Tensor    # [B,W] int64: the value it continues with
+
+
+def _flags(t, what, dev):
+    """uint8 view of a bool / uint8 tensor."""
+    if t.dtype == torch.bool:
+        t = t.view(torch.uint8)
+    elif t.dtype != torch.uint8:
+        raise _lib.CsError(f"{what} must be a bool or uint8 tensor, got {t.dtype}")
+    return t
+
+
+def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int, *, normalise: bool = True,
+                mask: Optional[torch.Tensor] = None, finished: Optional[torch.Tensor] = None,
+                end_token: Optional[int] = None) -> BeamStep:
+    """The ``width`` (1 .. 64) best continuations of every example, best first.
+
+    ``scores`` [B,K] float32 / float64 (None: zeros, float32): what the beams have so far; -inf: a beam that is not in use (the
+    first step of a search starts from one beam).  ``logits`` [B,K,V] float32 / bfloat16 / float16, the values adjacent in
+    memory, any strides of the other axes.  A continuation scores
+    ``scores + logits - logsumexp(logits)``, or ``scores + logits`` with ``normalise=False``, formed in 64 bits;
+    equal scores go to the lowest (beam, value).  ``mask`` (bool, broadcastable to [B,K,V]; True = allowed): what is not
+    allowed takes no part in the normaliser either and may hold anything.  ``finished`` [B,K] (bool): such a beam only
+    continues with ``end_token``, at its score; its logits are not read.  NaN and -inf are never chosen; a beam with a NaN or
+    +inf among its allowed logits has no continuations (``normalise``).  An example with fewer than ``width`` continuations
+    ends in score -inf, token -1 and the slot's own index as parent."""
+    if logits.dim() != 3:
+        raise _lib.CsError(f"logits must be [B,K,V], got {tuple(logits.shape)}")
+    B, K, V = logits.shape
+    dev = _lib.on_device(logits, scores, mask, finished)
+    if logits.dtype not in _lib.CS_TYPE or logits.dtype == torch.float64:
+        raise _lib.CsError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if scores is None:
+        out_type = torch.float32
+    else:
+        out_type = scores.dtype
+        if out_type not in (torch.float32, torch.float64):
+            raise _lib.CsError(f"scores must be float32 or float64, got {out_type}")
+        if scores.shape != (B, K):
+            raise _lib.CsError(f"scores must be [{B},{K}], got {tuple(scores.shape)}")
+        scores = scores.contiguous()
+    if logits.stride(2) != 1 and V > 1:
+        logits = logits.contiguous()
+    cfg = _lib.cs_beam_cfg(B, K, V, int(width), _lib.CS_TYPE[logits.dtype], _lib.CS_TYPE[out_type], int(normalise), 0)
+    cfg.logits_stride[:] = logits.stride()[:2]
+    if mask is not None:
+        mask = _flags(mask, "mask", dev).expand(B, K, V)
+        if mask.stride(2) != 1 and V > 1:
+            mask = mask.contiguous()
+        cfg.mask_stride[:] = mask.stride()[:2]
+    if finished is not None:
+        if end_token is None:
+            raise _lib.CsError("finished needs end_token")
+        finished = _flags(finished, "finished", dev)
+        if finished.shape != (B, K):
+            raise _lib.CsError(f"finished must be [{B},{K}], got {tuple(finished.shape)}")
+        finished = finished.contiguous()
+        cfg.end_token = int(end_token)
+    L = _lib.lib()
+    nbytes = L.cs_beam_select_workspace(C.byref(cfg))
+    if nbytes < 0:
+        raise _lib.CsError(f"libcsvae error: {L.cs_last_error().decode()}")
+    W = cfg.W
+    # the workspace is the call's own (calls on several streams and captured ones share nothing)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    new_scores = torch.empty(B, W, dtype=out_type, device=dev)
+    chosen = torch.empty(2, B, W, dtype=torch.int64, device=dev)
+    parents, tokens = chosen[0], chosen[1]
+    p = lambda t: None if t is None else t.data_ptr()
+    _lib.call_on(dev, L.cs_beam_select, C.byref(cfg), p(scores), logits.data_ptr(), p(mask), p(finished),
+                 new_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr(), nbytes)
+    return BeamStep(new_scores, parents, tokens)
+
+
+def _rows(t, axis):
+    """(outer, strides in bytes of (outer, example, chain), bytes of a row) of t[outer..., B, K, row...], or None if the
+    outer axes do not collapse into one stride or a row is not adjacent in memory."""
+    size = t.element_size()
+    row = 1
+    for n, s in zip(reversed(t.shape[axis + 2:]), reversed(t.stride()[axis + 2:])):
+        if n != 1 and s != row:
+            return None
+        row *= n
+    outer, stride = 1, 0
+    for n, s in zip(reversed(t.shape[:axis]), reversed(t.stride()[:axis])):
+        if n == 1:
+            continue
+        if outer == 1:
+            stride = s
+        elif s != stride * outer:
+            return None
+        outer *= n
+    return outer, (stride * size, t.stride(axis) * size, t.stride(axis + 1) * size), row * size
+
+
+def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: int = 0,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[..., b, w, ...] = states[..., b, parents[b, w], ...]`` for states of any type whose axes ``batch_dim`` and
+    ``batch_dim + 1`` are examples and chains: latents [B,K,Zd], a history [T,B,K,D] (``batch_dim=1``).
+
+    ``parents`` [B,W] int64; a parent outside [0,K) leaves its row of ``out`` as it was.  ``out=None`` returns a new tensor (a
+    row without a parent is zero there); ``out=states`` works in place (W = K <= 64): rows that keep their place are not
+    touched, so a search that leaves survivors where they are moves only what changed.  ``out`` elsewhere must not overlap
+    ``states``."""
+    if batch_dim < 0:
+        batch_dim += states.dim()
+    if not 0 <= batch_dim <= states.dim() - 2:
+        raise _lib.CsError("states need an example and a chain axis")
+    B, K = states.shape[batch_dim:batch_dim + 2]
+    if parents.dim() != 2 or parents.shape[0] != B or parents.dtype != torch.int64:
+        raise _lib.CsError(f"parents must be int64 [{B},W], got {parents.dtype} {tuple(parents.shape)}")
+    W = parents.shape[1]
+    shape = states.shape[:batch_dim + 1] + (W,) + states.shape[batch_dim + 2:]
+    if out is None:
+        out = torch.zeros(shape, dtype=states.dtype, device=states.device)
+    elif out.shape != shape or out.dtype != states.dtype:
+        raise _lib.CsError(f"out must be {states.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    dev = _lib.on_device(states, parents, out)
+    if out.numel() == 0:
+        return out
+    if K == 0:
+        raise _lib.CsError("no chains")
+    src, dst = _rows(states, batch_dim), _rows(out, batch_dim)
+    if dst is None:
+        raise _lib.CsError("out: rows must be adjacent in memory and the leading axes of one stride")
+    if src is None:   # (never in place: out has the same layout)
+        states = states.contiguous()
+        src = _rows(states, batch_dim)
+    parents = parents.contiguous()
+    i64x3 = C.c_int64 * 3
+    _lib.call_on(dev, _lib.lib().cs_beam_reorder, states.data_ptr(), out.data_ptr(), src[0], B, K, W, src[2],
+                 i64x3(*src[1]), i64x3(*dst[1]), parents.data_ptr())
+    return out

@@ -150,3 +150,114 @@ class ImputationHistoryQueue_with_restrictedavailability(object):
         if self.full:
             return (r + self.tail_idx + 1) % self.max_history_length
         return r
+
+
+class QuantisedHistory:
+    """Ring ``[T,B,K,D]`` of past states in 8 or 4 bits: quantised as they are written, read back by slot and chain.
+
+    ``fmt``: ``int8`` (a float32 scale for every ``group`` = 32, 64 or 128 consecutive values), ``mxfp8`` / ``mxfp4`` (e4m3 /
+    e2m1 elements of OCP Microscaling, groups of 32 with a power of two).  A state is one record, codes and scales
+    together (include/csvae.h, cs_qcache): a MiniBooNE state of 43 values takes 48, 48 or 32 bytes instead of 172.  A value
+    that is not finite reads as NaN (mxfp4: its whole group).  ``data`` is the ring [T,B,K,record] uint8, zeros at first (they
+    read as zeros, in int8; as zeros of the smallest scale in the others)."""
+
+    def __init__(self, max_history_length, batch_shape, fmt, group=None, device="cuda"):
+        if fmt not in _lib.CS_QFMT:
+            raise NotImplementedError(f"history format {fmt!r}")
+        group = (64 if fmt == "int8" else 32) if group is None else int(group)
+        self.max_history_length, self.batch_shape, self.fmt, self.group = int(max_history_length), tuple(batch_shape), fmt, group
+        B, K, D = self.batch_shape
+        self.record_bytes = int(_lib.lib().cs_qcache_record_bytes(_lib.CS_QFMT[fmt], group, D))
+        if self.record_bytes < 0 or self.max_history_length < 1 or K < 1:
+            raise _lib.CsError(f"no history of {self.max_history_length} states {self.batch_shape} as {fmt}, groups of {group}")
+        self.data = torch.zeros((self.max_history_length, B, K, self.record_bytes), dtype=torch.uint8, device=device)
+        self._desc = _lib.cs_qcache(None, self.max_history_length, B, K, D, _lib.CS_QFMT[fmt], group)
+
+    def _ring(self):
+        """The C description of the ring as it is now (``data`` may have been moved or replaced by one of its shape)."""
+        d = self.data
+        if d.shape != (self.max_history_length,) + self.batch_shape[:2] + (self.record_bytes,) or d.dtype != torch.uint8 \
+                or not d.is_contiguous():
+            raise _lib.CsError("data must stay a contiguous uint8 [T,B,K,record]")
+        self._desc.data = d.data_ptr()
+        return C.byref(self._desc)
+
+    def _int64(self, t, shape, what):
+        if t.dtype != torch.int64 or tuple(t.shape) != shape:
+            raise _lib.CsError(f"{what} must be int64 {list(shape)}, got {t.dtype} {list(t.shape)}")
+        return t.contiguous()
+
+    def write(self, X, start, counts=None):
+        """Quantise ``X`` [n,B,K,D] or [B,K,D] (float32 / bfloat16 / float16, any strides with D adjacent; n <= T) into the
+        slots ``start .. start + n - 1`` (mod T).  ``start``: an int, or an int64 tensor [B,K] with a position per chain (negative:
+        the chain is left out).  ``counts`` (int64 [B,K]): only the first ``counts[b,k]`` states of a chain are written; all
+        other records stay as they are."""
+        B, K, D = self.batch_shape
+        if X.dim() == 3:
+            X = X[None]
+        if X.dim() != 4 or tuple(X.shape[1:]) != (B, K, D):
+            raise _lib.CsError(f"states must be [n,{B},{K},{D}], got {list(X.shape)}")
+        if X.dtype not in _lib.CS_TYPE or X.dtype == torch.float64:
+            raise _lib.CsError(f"states must be float32, bfloat16 or float16, got {X.dtype}")
+        tensor = torch.is_tensor(start)
+        dev = _lib.on_device(self.data, X, start if tensor else None, counts)
+        if X.stride(3) != 1 and D > 1:
+            X = X.contiguous()
+        if tensor:
+            start = self._int64(start, (B, K), "start")
+        if counts is not None:
+            counts = self._int64(counts, (B, K), "counts")
+        _lib.call_on(dev, _lib.lib().cs_qcache_write, self._ring(), X.data_ptr(), _lib.CS_TYPE[X.dtype], X.shape[0],
+                     (C.c_int64 * 3)(*X.stride()[:3]), start.data_ptr() if tensor else None, 0 if tensor else int(start),
+                     None if counts is None else counts.data_ptr())
+
+    def read(self, slots, chains=None, *, dtype=torch.float32, out=None):
+        """``out[n,b,j] = state at slots[n,b,j] of chain chains[n,b,j]`` (None: of chain j) of example b, zeros where slot or
+        chain do not exist.  ``slots`` / ``chains`` int64 [N,B,J] or [B,J]; ``out`` [N,B,J,D] (or [B,J,D]): any strides with D
+        adjacent."""
+        B, K, D = self.batch_shape
+        single = slots.dim() == 2
+        if single:
+            slots = slots[None]
+            chains = None if chains is None else chains[None]
+            out = None if out is None else out[None]
+        if slots.dim() != 3 or slots.shape[1] != B or slots.dtype != torch.int64 or (chains is None and slots.shape[2] != K):
+            raise _lib.CsError(f"slots must be int64 [N,{B},{K}] (or [N,{B},J] with chains), got {slots.dtype} {list(slots.shape)}")
+        N, _, J = slots.shape
+        if chains is not None:
+            chains = self._int64(chains, (N, B, J), "chains")
+        slots = slots.contiguous()
+        out = self._out(out, (N, B, J, D), dtype)
+        if out.numel():
+            dev = _lib.on_device(self.data, slots, chains, out)
+            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring(), slots.data_ptr(), 0,
+                         None if chains is None else chains.data_ptr(), N, J, out.data_ptr(), _lib.CS_TYPE[out.dtype],
+                         (C.c_int64 * 3)(*out.stride()[:3]))
+        return out[0] if single else out
+
+    def read_steps(self, start, n, *, dtype=torch.float32, out=None):
+        """The states of all chains at the slots ``start .. start + n - 1`` (mod T): [n,B,K,D]."""
+        B, K, D = self.batch_shape
+        out = self._out(out, (int(n), B, K, D), dtype)
+        if out.numel():
+            dev = _lib.on_device(self.data, out)
+            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring(), None, int(start), None, int(n), K, out.data_ptr(),
+                         _lib.CS_TYPE[out.dtype], (C.c_int64 * 3)(*out.stride()[:3]))
+        return out
+
+    def _out(self, out, shape, dtype):
+        if out is None:
+            if dtype not in _lib.CS_TYPE or dtype == torch.float64:
+                raise _lib.CsError(f"states are read as float32, bfloat16 or float16, got {dtype}")
+            return torch.empty(shape, dtype=dtype, device=self.data.device)
+        if tuple(out.shape) != shape or out.dtype not in _lib.CS_TYPE or out.dtype == torch.float64 \
+                or (out.stride(3) != 1 and shape[3] > 1):
+            raise _lib.CsError(f"out must be float32, bfloat16 or float16 {list(shape)} with adjacent values")
+        return out
+
+    def reorder(self, parents, steps=None):
+        """The records of every chain follow ``parents`` [B,K] in place (``beam.reorder_states``), in the first ``steps`` slots
+        (None: all)."""
+        from .beam import reorder_states
+        data = self.data if steps is None else self.data[:int(steps)]
+        reorder_states(data, parents, batch_dim=1, out=data)
