@@ -17,14 +17,30 @@ namespace {
 
 constexpr int QC_LANE = 8;     // values a lane holds
 
+// n / d and n mod d for any 32-bit n by a multiplication (Granlund and Montgomery's round-up form): 64-bit divisions by
+// the sizes of a call cost several hundred instructions per lane, more than all else these kernels do.
+struct QcDiv {
+  uint32_t d, mul, shift;
+};
+QcDiv qc_div(int64_t d) {
+  uint32_t l = 0;
+  while (l < 32 && (1ull << l) < (uint64_t)d) ++l;
+  const uint64_t mul = ((1ull << 32) * ((1ull << l) - (uint64_t)d)) / (uint64_t)d + 1;
+  return QcDiv{(uint32_t)d, (uint32_t)mul, l};
+}
+__device__ __forceinline__ uint32_t qc_over(uint32_t n, const QcDiv& d) {
+  const uint32_t t = __umulhi(n, d.mul);
+  return d.shift == 0 ? n : (t + ((n - t) >> 1)) >> (d.shift - 1);
+}
+
 struct QcArgs {
   cs_qcache c;
   int64_t record;              // bytes
   int32_t code_bytes;          // of a record, rounded up to 4
   int32_t lanes;               // lanes of a row: groups * G / 8
   int32_t rows_per_block;
-  int64_t rows, chains;        // rows of the call; B * K (write) or B * J (read)
-  int32_t J;
+  uint32_t rows;               // rows of the call, below 2^31
+  QcDiv by_lanes, by_chains, by_inner, by_T;   // lanes; B * K (write) or B * J (read); K or J; T
   const void* x;               // write
   void* out;                   // read
   int64_t stride[3];
@@ -129,24 +145,46 @@ __device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale,
   for (int i = 0; i < QC_LANE; ++i) v[i] = scale == 255u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v[i], e);
 }
 
-// the slot of row r of a call (n steps of `chains` chains from `start` on); -1: not in the call
-__device__ __forceinline__ int64_t qc_slot(const QcArgs& a, int64_t i, int64_t chain) {
-  if (a.count && i >= a.count[chain]) return -1;
-  const int64_t s = a.start ? a.start[chain] : a.start0;
-  if (s < 0) return -1;
-  return (s % a.c.T + i) % a.c.T;
+// the slot of step i of a chain of a call that runs from `start` on; -1: not in the call
+__device__ __forceinline__ int32_t qc_slot(const QcArgs& a, uint32_t i, uint32_t chain) {
+  if (a.count && (int64_t)i >= a.count[chain]) return -1;
+  const uint32_t T = a.by_T.d;
+  uint32_t s = (uint32_t)a.start0;               // (below T)
+  if (a.start) {
+    const int64_t far = a.start[chain];
+    if (far < 0) return -1;
+    s = far < (int64_t)T ? (uint32_t)far : (uint32_t)(far % (int64_t)T);
+  }
+  s += i - qc_over(i, a.by_T) * T;
+  return (int32_t)(s >= T ? s - T : s);
+}
+
+// 8 values from / to addresses aligned to the type alone (the hardware takes any address)
+template <typename T>
+__device__ __forceinline__ void qc_load8(const T* p, float* v) {
+  T r[QC_LANE];
+  __builtin_memcpy(r, p, sizeof(r));
+#pragma unroll
+  for (int e = 0; e < QC_LANE; ++e) v[e] = qc_float(r[e]);
+}
+template <typename T>
+__device__ __forceinline__ void qc_store8(T* p, const float* v) {
+  T r[QC_LANE];
+#pragma unroll
+  for (int e = 0; e < QC_LANE; ++e) qc_store(r + e, v[e]);
+  __builtin_memcpy(p, r, sizeof(r));
 }
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
-  const int ry = threadIdx.x / a.lanes;
-  const int64_t row = (int64_t)blockIdx.x * a.rows_per_block + ry;
+  const int ry = (int)qc_over(threadIdx.x, a.by_lanes);
+  const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
   const bool live = ry < a.rows_per_block && row < a.rows;
-  const int64_t i = live ? row / a.chains : 0, chain = live ? row - i * a.chains : 0;
-  const int64_t slot = live ? qc_slot(a, i, chain) : -1;
-  const int64_t b = chain / a.c.K, k = chain - b * a.c.K;
+  const uint32_t i = live ? qc_over(row, a.by_chains) : 0, chain = live ? row - i * a.by_chains.d : 0;
+  const int32_t slot = live ? qc_slot(a, i, chain) : -1;
+  const uint32_t b = qc_over(chain, a.by_inner), k = chain - b * a.by_inner.d;
   const T* x = (const T*)a.x + i * a.stride[0] + b * a.stride[1] + k * a.stride[2];
-  char* rec = (char*)a.c.data + ((slot < 0 ? 0 : slot) * a.chains + chain) * a.record;
+  char* rec = (char*)a.c.data + ((int64_t)(slot < 0 ? 0 : slot) * a.by_chains.d + chain) * a.record;
   const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
   // (lanes of a row: a multiple of the lanes of a group, which divide 64; whole groups of lanes take part or none)
   for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
@@ -154,8 +192,12 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
     float v[QC_LANE];
     float top = 0.0f;
     bool fine = true;
+    if (slot >= 0 && d0 + QC_LANE <= D) {
+      qc_load8(x + d0, v);
+    } else {
 #pragma unroll
-    for (int e = 0; e < QC_LANE; ++e) v[e] = slot >= 0 && d0 + e < D ? qc_float(x[d0 + e]) : 0.0f;
+      for (int e = 0; e < QC_LANE; ++e) v[e] = slot >= 0 && d0 + e < D ? qc_float(x[d0 + e]) : 0.0f;
+    }
 #pragma unroll
     for (int e = 0; e < QC_LANE; ++e) {
       const float m = __builtin_fabsf(v[e]);
@@ -184,11 +226,11 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
-  const int ry = threadIdx.x / a.lanes;
-  const int64_t row = (int64_t)blockIdx.x * a.rows_per_block + ry;
+  const int ry = (int)qc_over(threadIdx.x, a.by_lanes);
+  const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
   if (ry >= a.rows_per_block || row >= a.rows) return;
-  const int64_t i = row / a.chains, chain = row - i * a.chains;
-  const int64_t b = chain / a.J, j = chain - b * a.J;
+  const uint32_t i = qc_over(row, a.by_chains), chain = row - i * a.by_chains.d;
+  const uint32_t b = qc_over(chain, a.by_inner), j = chain - b * a.by_inner.d;
   const int64_t slot = a.slots ? a.slots[row] : qc_slot(a, i, chain);
   const int64_t k = a.from ? a.from[row] : j;
   const bool there = slot >= 0 && slot < a.c.T && k >= 0 && k < a.c.K;
@@ -207,9 +249,13 @@ __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
     }
     float v[QC_LANE];
     qc_decode<FMT>(codes, scale, v);
+    if (d0 + QC_LANE <= D) {
+      qc_store8(out + d0, v);
+    } else {
 #pragma unroll
-    for (int e = 0; e < QC_LANE; ++e)
-      if (d0 + e < D) qc_store(out + d0 + e, v[e]);
+      for (int e = 0; e < QC_LANE; ++e)
+        if (d0 + e < D) qc_store(out + d0 + e, v[e]);
+    }
   }
 }
 
@@ -220,7 +266,7 @@ int64_t code_bytes_of(int fmt, int64_t D) {
 
 int check_qcache(const cs_qcache* c) {
   CS_REQUIRE(c, "null argument");
-  CS_REQUIRE(c->T >= 1 && c->B >= 0 && c->K >= 1 && c->D >= 1, "bad sizes");
+  CS_REQUIRE(c->T >= 1 && c->T <= INT32_MAX && c->B >= 0 && c->K >= 1 && c->D >= 1, "bad sizes");
   CS_REQUIRE(c->fmt == CS_QFMT_INT8 || c->fmt == CS_QFMT_MXFP8 || c->fmt == CS_QFMT_MXFP4, "unknown format");
   if (c->fmt == CS_QFMT_INT8) CS_REQUIRE(c->group == 32 || c->group == 64 || c->group == 128, "int8: groups of 32, 64 or 128");
   else CS_REQUIRE(c->group == 32, "mxfp8 / mxfp4: groups of 32");
@@ -241,18 +287,24 @@ void launch_type(const QcArgs& a, int type, dim3 grid, hipStream_t st) {
   }
 }
 
+// n steps of B * inner rows
 template <bool WRITE>
-int launch(QcArgs& a, int type, hipStream_t st) {
+int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStream_t st) {
   const cs_qcache& c = a.c;
+  CS_REQUIRE(c.B <= INT32_MAX / inner && n <= INT32_MAX / (c.B * inner), "2^31 states or more in one call");
+  a.rows = (uint32_t)(n * c.B * inner);
+  a.by_chains = qc_div(c.B * inner);
+  a.by_inner = qc_div(inner);
+  a.by_T = qc_div(c.T);
+  a.start0 = start0 % c.T;
   CS_REQUIRE(type == CS_TYPE_F32 || type == CS_TYPE_BF16 || type == CS_TYPE_F16, "states are float32, bfloat16 or float16");
   CS_REQUIRE(((uintptr_t)c.data & 15) == 0, "the ring must be 16-byte aligned");
   a.record = cs_qcache_record_bytes(c.fmt, c.group, c.D);
   a.code_bytes = (int32_t)code_bytes_of(c.fmt, c.D);
   a.lanes = (c.D + c.group - 1) / c.group * (c.group / QC_LANE);
+  a.by_lanes = qc_div(a.lanes);
   a.rows_per_block = a.lanes >= 256 ? 1 : 256 / a.lanes;
-  const int64_t blocks = (a.rows + a.rows_per_block - 1) / a.rows_per_block;
-  CS_REQUIRE(blocks <= INT32_MAX, "too many states for one call");
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid((a.rows + a.rows_per_block - 1) / a.rows_per_block);
   if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, grid, st);
   else if (c.fmt == CS_QFMT_MXFP8) launch_type<WRITE, CS_QFMT_MXFP8>(a, type, grid, st);
   else launch_type<WRITE, CS_QFMT_MXFP4>(a, type, grid, st);
@@ -278,11 +330,9 @@ extern "C" int cs_qcache_write(const cs_qcache* c, const void* X, int32_t x_type
   CS_REQUIRE(c->data && X && x_stride, "null argument");
   QcArgs a = {};
   a.c = *c;
-  a.chains = c->B * c->K;
-  a.rows = n * a.chains;
-  a.x = X; a.start = start; a.start0 = start0; a.count = count;
+  a.x = X; a.start = start; a.count = count;
   for (int i = 0; i < 3; ++i) a.stride[i] = x_stride[i];
-  return launch<true>(a, x_type, (hipStream_t)stream);
+  return launch<true>(a, n, c->K, start ? 0 : start0, x_type, (hipStream_t)stream);
 }
 
 extern "C" int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t start0, const int64_t* chains, int64_t N, int32_t J,
@@ -295,10 +345,7 @@ extern "C" int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t 
   CS_REQUIRE(c->data && out && out_stride, "null argument");
   QcArgs a = {};
   a.c = *c;
-  a.chains = c->B * J;
-  a.rows = N * a.chains;
-  a.J = J;
-  a.out = out; a.slots = slots; a.start0 = start0; a.from = chains;
+  a.out = out; a.slots = slots; a.from = chains;
   for (int i = 0; i < 3; ++i) a.stride[i] = out_stride[i];
-  return launch<false>(a, out_type, (hipStream_t)stream);
+  return launch<false>(a, N, J, slots ? 0 : start0, out_type, (hipStream_t)stream);
 }
