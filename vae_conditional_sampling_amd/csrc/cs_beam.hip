@@ -18,7 +18,7 @@ constexpr int BM_LANE = 32;            // logits a lane holds
 constexpr int BM_STRETCH = 64 * BM_LANE;
 constexpr int BM_LIST = 256;           // preselected logits of a stretch
 constexpr int BM_MAXK = 2048;
-constexpr int BM_JOIN = 256;           // threads that join an example
+constexpr int BM_JOIN = 1024;          // threads that join an example, at most
 constexpr float BM_LOWEST = -3.402823466e+38f;
 
 struct BmItem { float x; int32_t v; };           // v < 0: none
@@ -95,6 +95,32 @@ __device__ __forceinline__ double bm_wave_sum(double v) {
   return v;
 }
 
+// 2^(j / 32)
+__device__ const double bm_pow32[32] = {
+    1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+
+// exp(d) for -700 <= d <= 0 as 2^n 2^(j/32) exp(r), 32 n + j the integer nearest to 32 d / ln 2 and |r| <= ln 2 / 64, exp(r) by
+// its Taylor polynomial of degree 4 (remainder r^5 / 120 < 1.3e-12): the table-driven method of Tang (1989).  Adding
+// 1.5 * 2^52 leaves the integer in the low word.  The table lies in LDS: 32 entries of 8 bytes fill the 64 banks once, so
+// no two of them meet in a bank.
+__device__ __forceinline__ double bm_exp(double d, const double* pow32) {
+  constexpr double MAGIC = 6755399441055744.0;
+  const double z = __builtin_fma(d, 46.16624130844683, MAGIC);   // 32 / ln 2
+  const int nj = (int)(uint32_t)(uint64_t)__double_as_longlong(z);
+  const double r = __builtin_fma(z - MAGIC, -0.02166084939249829, d);   // ln 2 / 32
+  const double t = pow32[nj & 31];
+  const double tn = __hiloint2double(__double2hiint(t) + ((nj & ~31) << 15), __double2loint(t));
+  const double p = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
+  return tn * p;
+}
+
 // The largest key that at least W lanes reach with theirs (0 if fewer than W lanes have one): bits from the top.
 template <typename U>
 __device__ __forceinline__ U bm_wave_threshold(U key, int W) {
@@ -111,6 +137,9 @@ template <typename T, bool MASK>
 __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   constexpr int N = BmElem<T>::N;      // logits in 16 bytes
   __shared__ BmItem s_list[4][BM_LIST];
+  __shared__ double s_pow[32];
+  if (threadIdx.x < 32) s_pow[threadIdx.x] = bm_pow32[threadIdx.x];
+  __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t item = (int64_t)blockIdx.x * 4 + wave;
   const int64_t rows = (int64_t)a.c.B * a.c.K;
@@ -158,20 +187,32 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
       if (top == __builtin_inff()) {
         sum = __builtin_nan("");
       } else {
-        const double m = top > -__builtin_inff() ? (double)top : 0.0;
+        uint64_t nan = 0;
 #pragma unroll
-        for (int i = 0; i < BM_LANE; ++i) sum += exp((double)x[i] - m);   // (a NaN makes the sum one)
-        sum = bm_wave_sum(sum);
+        for (int i = 0; i < BM_LANE; ++i) nan |= __ballot(x[i] != x[i]);
+        if (top > -__builtin_inff()) {
+          const double m = (double)top;
+#pragma unroll
+          for (int i = 0; i < BM_LANE; ++i) sum += bm_exp(fmax((double)x[i] - m, -690.0), s_pow);   // (less than 1e-299)
+          sum = bm_wave_sum(sum);
+        }
+        if (nan) sum = __builtin_nan("");
       }
     }
     // everything from the W-th largest of the lanes' best on is a candidate
     const uint32_t tk = bm_wave_threshold<uint32_t>(best > -__builtin_inff() ? bm_key(best) : 0u, W);
     float t = tk ? fmaxf(bm_value(tk), BM_LOWEST) : BM_LOWEST;
-    int cnt = 0;
+    const int32_t v_lane = base + lane * N;
 #pragma unroll
-    for (int i = 0; i < BM_LANE; ++i) cnt += __popcll(__ballot(x[i] >= t));
-    bool refined = false;
-    if (cnt > BM_LIST) {   // many equal or ascending values: the W-th largest of all, bit by bit
+    for (int i = 0; i < BM_LANE; ++i) {
+      const uint64_t m = __ballot(x[i] >= t);
+      if (m) {
+        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        if (x[i] >= t && at < BM_LIST) s_list[wave][at] = BmItem{x[i] + 0.0f, v_lane + (i / N) * 64 * N + i % N};
+        n += __popcll(m);
+      }
+    }
+    if (n > BM_LIST) {   // many equal or ascending values: the W-th largest of all, bit by bit
       uint32_t u = 0;
       for (int bit = 31; bit >= 0; --bit) {
         const float f = bm_value(u | (1u << bit));   // (patterns of NaN reach nothing)
@@ -181,17 +222,14 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
         if (c >= W) u |= 1u << bit;
       }
       t = bm_value(u);
-      refined = true;
-    }
-    const int32_t v_lane = base + lane * N;
+      n = 0;
 #pragma unroll
-    for (int i = 0; i < BM_LANE; ++i) {
-      const bool take = refined ? x[i] > t : x[i] >= t;
-      const uint64_t m = __ballot(take);
-      if (take) s_list[wave][n + __popcll(m & ((1ull << lane) - 1))] = BmItem{x[i] + 0.0f, v_lane + (i / N) * 64 * N + i % N};
-      n += __popcll(m);
-    }
-    if (refined) {   // of those equal to the W-th the first ones
+      for (int i = 0; i < BM_LANE; ++i) {
+        const uint64_t m = __ballot(x[i] > t);
+        if (x[i] > t) s_list[wave][n + __popcll(m & ((1ull << lane) - 1))] = BmItem{x[i] + 0.0f, v_lane + (i / N) * 64 * N + i % N};
+        n += __popcll(m);
+      }
+      // of those equal to the W-th the first ones
 #pragma unroll
       for (int j = 0; j < BM_LANE / N; ++j) {
         int mine = 0;
@@ -239,12 +277,16 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
   __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = blockDim.x, waves = threads >> 6;
   const int64_t b = blockIdx.x;
   const int K = a.c.K, W = a.c.W, C = a.stretches;
   const int64_t V = a.c.V;
+  const int64_t total = (int64_t)K * C;
+  const BmItem* item = a.item + b * total * W;
+  // (asked for before the normalisers are formed)
+  const BmItem first = tid < total ? item[(int64_t)tid * W] : BmItem{0.0f, -1};
   if (tid == 0) s_n = 0;
-  for (int k = wave; k < K; k += BM_JOIN / 64) {
+  for (int k = wave; k < K; k += waves) {
     const int64_t row = b * K + k;
     double before = 0.0;
     if (a.scores) before = a.c.scores_type == CS_TYPE_F64 ? ((const double*)a.scores)[row] : (double)((const float*)a.scores)[row];
@@ -267,11 +309,9 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   }
   __syncthreads();
   // the W-th largest among the stretches' best bounds the result from below
-  const int64_t total = (int64_t)K * C;
-  const BmItem* item = a.item + b * total * W;
   uint64_t best = 0;
-  for (int64_t g = tid; g < total; g += BM_JOIN) {
-    const BmItem i = item[g * W];
+  for (int64_t g = tid; g < total; g += threads) {
+    const BmItem i = g == tid ? first : item[g * W];
     if (i.v >= 0) {
       const uint64_t key = bm_key64((double)i.x + s_beam[g / C]);
       best = key > best ? key : best;
@@ -281,8 +321,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   if (lane == 0) s_wave[wave] = t_wave;
   __syncthreads();
   uint64_t t = 1;
-  for (int w = 0; w < BM_JOIN / 64; ++w) t = s_wave[w] > t ? s_wave[w] : t;
-  for (int64_t g = tid; g < total; g += BM_JOIN) {
+  for (int w = 0; w < waves; ++w) t = s_wave[w] > t ? s_wave[w] : t;
+  for (int64_t g = tid; g < total; g += threads) {
     const int k = (int)(g / C);
     for (int r = 0; r < W; ++r) {          // sorted: the first that falls short ends the stretch
       const BmItem i = item[g * W + r];
@@ -304,14 +344,14 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   };
   const int n = s_n;
   if (n <= cap) {
-    for (int i = tid; i < n; i += BM_JOIN) {
+    for (int i = tid; i < n; i += threads) {
       const uint64_t key = s_key[i];
       const int64_t at = s_at[i];
       int rank = 0;
       for (int j = 0; j < n; ++j) rank += s_key[j] > key || (s_key[j] == key && s_at[j] < at);
       if (rank < W) put(rank, key, at);
     }
-    for (int w = n + tid; w < W; w += BM_JOIN) put(w, 0, 0);
+    for (int w = n + tid; w < W; w += threads) put(w, 0, 0);
     return;
   }
   // many equal scores: the results one by one, each the best of what comes after the one before
@@ -320,7 +360,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   for (int w = 0; w < W; ++w) {
     uint64_t key = 0;
     int64_t at = 0;
-    for (int64_t g = tid; g < total; g += BM_JOIN) {
+    for (int64_t g = tid; g < total; g += threads) {
       const int k = (int)(g / C);
       for (int r = 0; r < W; ++r) {
         const BmItem i = item[g * W + r];
@@ -339,7 +379,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     if (lane == 0) { s_wave[wave] = key; s_wave_at[wave] = at; }
     __syncthreads();
     key = s_wave[0]; at = s_wave_at[0];
-    for (int v = 1; v < BM_JOIN / 64; ++v)
+    for (int v = 1; v < waves; ++v)
       if (s_wave[v] > key || (s_wave[v] == key && s_wave_at[v] < at)) { key = s_wave[v]; at = s_wave_at[v]; }
     if (tid == 0) put(w, key, at);
     last = key ? key : 0;
@@ -400,7 +440,10 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   // a place for W candidates of each of W stretches, up to 32 KB
   int cap = c->W * c->W;
   cap = cap < 256 ? 256 : cap > 2048 ? 2048 : cap;
-  hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(BM_JOIN), (size_t)(((c->K * 8 + 15) & ~15) + cap * 16), st, a,
+  // a thread per stretch, as far as that goes
+  const int64_t total = (int64_t)c->K * a.stretches;
+  const int threads = total <= 64 && c->K <= 4 ? 64 : total <= 256 ? 256 : BM_JOIN;
+  hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads), (size_t)(((c->K * 8 + 15) & ~15) + cap * 16), st, a,
                      cap);
   CS_HIP(hipGetLastError());
   return CS_OK;
