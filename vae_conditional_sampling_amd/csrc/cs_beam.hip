@@ -3,36 +3,34 @@
 //
 // Selection.  s[k,v] = logits[k,v] + (scores[k] - lse[k]), lse the log of the sum of exponentials of the allowed logits
 // of beam k: the W largest over (k,v), ties to the lowest k*V + v.  One pass over the logits: a wavefront holds a
-// stretch of 2048 of one beam in registers (32 per lane), leaves their maximum, their sum of exponentials relative to it
-// and their W best (sorted) in the workspace; a workgroup per example then joins the stretches of every beam, turns the
+// stretch of one beam in registers (LANE values per lane), leaves their sum of exponentials and those of them that can
+// be among its W best in the workspace; a workgroup per example then joins the stretches of every beam, turns the
 // kept logits into scores and takes the W best of them.  The normaliser joins before scores of different beams are
-// compared, so within a beam a stretch's candidates can be ordered by their logits alone.  Sums and scores are held in
+// compared, so within a beam a stretch's candidates can be chosen by their logits alone.  Sums and scores are held in
 // 64 bits: two beams' candidates are often closer than float32 sums of 10^5 terms are exact, and the indices are to be
 // those of the definition.
 #include "cs_common.h"
 
 namespace {
 
-constexpr int BM_MAXW = 64;            // candidates per example and per stretch: a lane each
-constexpr int BM_LANE = 32;            // logits a lane holds
-constexpr int BM_STRETCH = 64 * BM_LANE;
-constexpr int BM_LIST = 256;           // preselected logits of a stretch
+constexpr int BM_MAXW = 64;            // candidates per example: a lane each
 constexpr int BM_MAXK = 2048;
 constexpr int BM_JOIN = 1024;          // threads that join an example, at most
 constexpr float BM_LOWEST = -3.402823466e+38f;
 
-struct BmItem { float x; int32_t v; };           // v < 0: none
-struct BmStat { double sum; float top; float pad; };
+struct BmItem { float x; int32_t v; };
+// of a stretch: the sum of exp(x - ref), the largest logit, the number of kept ones
+struct BmStat { double ref, sum; float top; int32_t n; };
 
 struct BmArgs {
   cs_beam_cfg c;
   const void *scores, *logits;
   const uint8_t *mask, *finished;
   BmStat* stat;     // [B*K*stretches]
-  BmItem* item;     // [B*K*stretches][W]
+  BmItem* item;     // [B*K*stretches][keep]
   void* out_scores;
   int64_t *parents, *tokens;
-  int32_t stretches;
+  int32_t stretches, keep;
 };
 
 __device__ __forceinline__ uint32_t bm_key(float v) {
@@ -95,177 +93,195 @@ __device__ __forceinline__ double bm_wave_sum(double v) {
   return v;
 }
 
-// 2^(j / 32)
-__device__ const double bm_pow32[32] = {
-    1, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
-    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
-    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
-    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
-    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
-    1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072,
-    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+// 2^(j / 64)
+__device__ const double bm_pow64[64] = {
+    1, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.1023825833078409, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.2021567314527031, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.2553807570246911, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.3396675240533029,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.5590044002378369, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.6457554781539649, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.7186192981224779, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509};
 
-// exp(d) for -700 <= d <= 0 as 2^n 2^(j/32) exp(r), 32 n + j the integer nearest to 32 d / ln 2 and |r| <= ln 2 / 64, exp(r) by
-// its Taylor polynomial of degree 4 (remainder r^5 / 120 < 1.3e-12): the table-driven method of Tang (1989).  Adding
-// 1.5 * 2^52 leaves the integer in the low word.  The table lies in LDS: 32 entries of 8 bytes fill the 64 banks once, so
-// no two of them meet in a bank.
-__device__ __forceinline__ double bm_exp(double d, const double* pow32) {
+// exp(d) 2^-n0 as 2^(n - n0) 2^(j/64) exp(r), 64 n + j the integer nearest to 64 d / ln 2 and |r| <= ln 2 / 128, exp(r) by its
+// Taylor polynomial of degree 3 (remainder r^4 / 24 < 3.6e-11): the table-driven method of Tang (1989).  Adding 1.5 * 2^52
+// leaves the integer in the low word.  The table lies in the lanes' registers and is read by ds_bpermute, which takes the
+// lane from the index's low 6 bits by itself; its high words have j << 14 and n0 << 20 taken off beforehand, so one shift and
+// addition of the whole integer puts the exponent right.
+struct BmPow {
+  int hi, lo;
+  __device__ __forceinline__ BmPow(int lane, int n0) {
+    const double t = bm_pow64[lane];
+    hi = __double2hiint(t) - (lane << 14) - (n0 << 20);
+    lo = __double2loint(t);
+  }
+};
+__device__ __forceinline__ double bm_add_exp(double sum, double d, const BmPow& pow) {
   constexpr double MAGIC = 6755399441055744.0;
-  const double z = __builtin_fma(d, 46.16624130844683, MAGIC);   // 32 / ln 2
-  const int nj = (int)(uint32_t)(uint64_t)__double_as_longlong(z);
-  const double r = __builtin_fma(z - MAGIC, -0.02166084939249829, d);   // ln 2 / 32
-  const double t = pow32[nj & 31];
-  const double tn = __hiloint2double(__double2hiint(t) + ((nj & ~31) << 15), __double2loint(t));
-  const double p = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
-  return tn * p;
+  const double z = __builtin_fma(d, 92.33248261689366, MAGIC);
+  const int nj = __double2loint(z);
+  const double r = __builtin_fma(z - MAGIC, -0.010830424696249145, d);
+  const int hi = __builtin_amdgcn_ds_bpermute(nj << 2, pow.hi) + (nj << 14), lo = __builtin_amdgcn_ds_bpermute(nj << 2, pow.lo);
+  const double p = __builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 6, 0.5), r, 1.0), r, 1.0);
+  return __builtin_fma(__hiloint2double(hi, lo), p, sum);
 }
 
-// The largest key that at least W lanes reach with theirs (0 if fewer than W lanes have one): bits from the top.
-template <typename U>
-__device__ __forceinline__ U bm_wave_threshold(U key, int W) {
-  U t = 0;
-  for (int bit = (int)sizeof(U) * 8 - 1; bit >= 0; --bit) {
-    const U u = t | ((U)1 << bit);
+// The largest key, as far as its leading BITS bits say, that at least W lanes reach with theirs; 0 if fewer than W lanes
+// have one.  A bound that is a little low only lets a few more candidates through.
+template <int BITS>
+__device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = 31; bit > 31 - BITS; --bit) {
+    const uint32_t u = t | (1u << bit);
     if (__popcll(__ballot(key >= u)) >= W) t = u;
   }
   return t;
 }
 
 // One wavefront per stretch.
-template <typename T, bool MASK>
+template <typename T, bool MASK, int LANE>
 __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   constexpr int N = BmElem<T>::N;      // logits in 16 bytes
-  __shared__ BmItem s_list[4][BM_LIST];
-  __shared__ double s_pow[32];
-  if (threadIdx.x < 32) s_pow[threadIdx.x] = bm_pow32[threadIdx.x];
-  __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  constexpr float INF = __builtin_inff();
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = (int64_t)a.c.B * a.c.K;
-  const bool live = item < rows * a.stretches;
-  const int64_t row = live ? item / a.stretches : 0;
-  const int32_t base = live ? (int32_t)(item - row * a.stretches) * BM_STRETCH : 0;
+  if (item >= rows * a.stretches) return;
+  const int64_t row = item / a.stretches;
+  const int32_t base = (int32_t)(item - row * a.stretches) * (64 * LANE);
   const int64_t b = row / a.c.K, k = row - b * a.c.K;
-  const int W = a.c.W;
-  const bool finished = live && a.finished && a.finished[row];
+  const int W = a.c.W, keep = a.keep;
   const int32_t V = (int32_t)a.c.V;
-  int n = 0;                           // entries of the list (the same in every lane)
-  float top = -__builtin_inff();
-  double sum = 0.0;
-  if (finished) {                      // its one candidate keeps the beam's score; its logits are not read
-    if (lane == 0 && base == 0) s_list[wave][0] = BmItem{0.0f, (int32_t)a.c.end_token};
-    n = base == 0 ? 1 : 0;
-  } else if (live) {
-    const T* p = (const T*)a.logits + b * a.c.logits_stride[0] + k * a.c.logits_stride[1];
-    const uint8_t* mk = MASK ? a.mask + b * a.c.mask_stride[0] + k * a.c.mask_stride[1] : nullptr;
-    float x[BM_LANE];
-#pragma unroll
-    for (int j = 0; j < BM_LANE / N; ++j) {
-      const int32_t v0 = base + (j * 64 + lane) * N;
-      if (v0 + N <= V) {
-        uint32_t r[4];
-        __builtin_memcpy(r, p + v0, 16);
-        BmElem<T>::widen(r, x + j * N);
-        if (MASK) {
-          uint8_t m[N];
-          __builtin_memcpy(m, mk + v0, N);
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[j * N + e] = m[e] ? x[j * N + e] : -__builtin_inff();
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          x[j * N + e] = v0 + e < V && (!MASK || mk[v0 + e]) ? BmElem<T>::one(p + v0 + e) : -__builtin_inff();
-      }
+  BmItem* out = a.item + item * keep;
+  if (a.finished && a.finished[row]) {   // its one candidate keeps the beam's score; its logits are not read
+    if (lane == 0) {
+      a.stat[item] = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
+      if (base == 0) out[0] = BmItem{0.0f, (int32_t)a.c.end_token};
     }
-    float best = -__builtin_inff();
+    return;
+  }
+  const T* p = (const T*)a.logits + b * a.c.logits_stride[0] + k * a.c.logits_stride[1];
+  const uint8_t* mk = MASK ? a.mask + b * a.c.mask_stride[0] + k * a.c.mask_stride[1] : nullptr;
+  float x[LANE];
 #pragma unroll
-    for (int i = 0; i < BM_LANE; ++i) best = fmaxf(best, x[i]);   // (a NaN is passed over)
-    top = bm_wave_max(best);
-    if (a.c.normalise) {
-      if (top == __builtin_inff()) {
-        sum = __builtin_nan("");
-      } else {
-        uint64_t nan = 0;
+  for (int j = 0; j < LANE / N; ++j) {
+    const int32_t v0 = base + (j * 64 + lane) * N;
+    if (v0 + N <= V) {
+      uint32_t r[4];
+      __builtin_memcpy(r, p + v0, 16);
+      BmElem<T>::widen(r, x + j * N);
+      if (MASK) {
+        uint8_t m[N];
+        __builtin_memcpy(m, mk + v0, N);
 #pragma unroll
-        for (int i = 0; i < BM_LANE; ++i) nan |= __ballot(x[i] != x[i]);
-        if (top > -__builtin_inff()) {
-          const double m = (double)top;
-#pragma unroll
-          for (int i = 0; i < BM_LANE; ++i) sum += bm_exp(fmax((double)x[i] - m, -690.0), s_pow);   // (less than 1e-299)
-          sum = bm_wave_sum(sum);
-        }
-        if (nan) sum = __builtin_nan("");
+        for (int e = 0; e < N; ++e) x[j * N + e] = m[e] ? x[j * N + e] : -INF;
       }
-    }
-    // everything from the W-th largest of the lanes' best on is a candidate
-    const uint32_t tk = bm_wave_threshold<uint32_t>(best > -__builtin_inff() ? bm_key(best) : 0u, W);
-    float t = tk ? fmaxf(bm_value(tk), BM_LOWEST) : BM_LOWEST;
-    const int32_t v_lane = base + lane * N;
+    } else {
 #pragma unroll
-    for (int i = 0; i < BM_LANE; ++i) {
-      const uint64_t m = __ballot(x[i] >= t);
-      if (m) {
-        const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-        if (x[i] >= t && at < BM_LIST) s_list[wave][at] = BmItem{x[i] + 0.0f, v_lane + (i / N) * 64 * N + i % N};
-        n += __popcll(m);
-      }
-    }
-    if (n > BM_LIST) {   // many equal or ascending values: the W-th largest of all, bit by bit
-      uint32_t u = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const float f = bm_value(u | (1u << bit));   // (patterns of NaN reach nothing)
-        int c = 0;
-#pragma unroll
-        for (int i = 0; i < BM_LANE; ++i) c += __popcll(__ballot(x[i] >= f));
-        if (c >= W) u |= 1u << bit;
-      }
-      t = bm_value(u);
-      n = 0;
-#pragma unroll
-      for (int i = 0; i < BM_LANE; ++i) {
-        const uint64_t m = __ballot(x[i] > t);
-        if (x[i] > t) s_list[wave][n + __popcll(m & ((1ull << lane) - 1))] = BmItem{x[i] + 0.0f, v_lane + (i / N) * 64 * N + i % N};
-        n += __popcll(m);
-      }
-      // of those equal to the W-th the first ones
-#pragma unroll
-      for (int j = 0; j < BM_LANE / N; ++j) {
-        int mine = 0;
-#pragma unroll
-        for (int e = 0; e < N; ++e) mine += x[j * N + e] == t;
-        int incl = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-          const int other = __shfl_up(incl, o);
-          if (lane >= o) incl += other;
-        }
-        int at = n + incl - mine;
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (x[j * N + e] == t) {
-            if (at < W) s_list[wave][at] = BmItem{t + 0.0f, v_lane + j * 64 * N + e};
-            ++at;
-          }
-        n += __shfl(incl, 63);
-      }
-      n = n < W ? n : W;
+      for (int e = 0; e < N; ++e)
+        x[j * N + e] = v0 + e < V && (!MASK || mk[v0 + e]) ? BmElem<T>::one(p + v0 + e) : -INF;
     }
   }
-  __syncthreads();
-  if (!live) return;
-  if (lane == 0) a.stat[item] = BmStat{sum, top, 0.0f};
-  BmItem* out = a.item + item * W;
-  for (int i = lane; i < n; i += 64) {
-    const BmItem mine = s_list[wave][i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const BmItem o = s_list[wave][j];
-      rank += o.x > mine.x || (o.x == mine.x && o.v < mine.v);
-    }
-    if (rank < W) out[rank] = mine;
+  float best = -INF, least = INF;      // (a NaN is passed over)
+#pragma unroll
+  for (int i = 0; i < LANE; ++i) {
+    best = fmaxf(best, x[i]);
+    least = fminf(least, x[i]);
   }
-  for (int i = n + lane; i < W; i += 64) out[i] = BmItem{0.0f, -1};
+  const float top = bm_wave_max(best);
+  double ref = 0.0, sum = 0.0, sum1 = 0.0;
+  if (a.c.normalise) {
+    least = -bm_wave_max(-least);
+    if (top < 8192.0f && least > -8192.0f && top - least < 600.0f) {
+      // no exponent can leave its range (a NaN makes the sum one)
+      const int n0 = (int)__builtin_rintf(top * 1.44269504f);
+      const BmPow pow(lane, n0);
+      ref = n0 * 0.6931471805599453;
+#pragma unroll
+      for (int i = 0; i < LANE; i += 2) {
+        sum = bm_add_exp(sum, (double)x[i], pow);
+        sum1 = bm_add_exp(sum1, (double)x[i + 1], pow);
+      }
+    } else {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < LANE; ++i) nan = nan || x[i] != x[i];
+      if (top > -INF) {
+        const BmPow pow(lane, 0);
+        ref = (double)top;
+        // (less than exp(-690) counts as that; of an infinite top every difference is NaN or -inf)
+#pragma unroll
+        for (int i = 0; i < LANE; ++i) sum = bm_add_exp(sum, fmax((double)x[i] - ref, -690.0), pow);
+      }
+      if (__ballot(nan) || top == INF) sum = __builtin_nan("");
+    }
+    sum = bm_wave_sum(sum + sum1);
+  }
+  // everything from the W-th largest of the lanes' best on is kept
+  const uint32_t tk = bm_wave_threshold<16>(best > -INF ? bm_key(best) : 0u, W);
+  float t = tk >= bm_key(BM_LOWEST) ? bm_value(tk) : BM_LOWEST;
+  const int32_t v_lane = base + lane * N;
+  int n = 0;                           // (the same in every lane)
+#pragma unroll
+  for (int i = 0; i < LANE; ++i) {
+    const uint64_t m = __ballot(x[i] >= t);
+    if (m) {
+      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      n += __popcll(m);
+      if (n <= keep && x[i] >= t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
+    }
+  }
+  if (n > keep) {   // many equal or ascending values: the W-th largest of all, bit by bit
+    uint32_t u = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const float f = bm_value(u | (1u << bit));   // (patterns of NaN reach nothing)
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < LANE; ++i) c += __popcll(__ballot(x[i] >= f));
+      if (c >= W) u |= 1u << bit;
+    }
+    t = bm_value(u);
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < LANE; ++i) {
+      const uint64_t m = __ballot(x[i] > t);
+      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      if (x[i] > t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
+      n += __popcll(m);
+    }
+    // of those equal to it the first ones
+#pragma unroll
+    for (int j = 0; j < LANE / N; ++j) {
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) mine += x[j * N + e] == t;
+      int incl = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int other = __shfl_up(incl, o);
+        if (lane >= o) incl += other;
+      }
+      int at = n + incl - mine;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (x[j * N + e] == t) {
+          if (at < W) out[at] = BmItem{t, v_lane + j * 64 * N + e};
+          ++at;
+        }
+      n += __shfl(incl, 63);
+    }
+    n = n < W ? n : W;
+  }
+  if (lane == 0) a.stat[item] = BmStat{ref, sum, top, n};
 }
 
 // One workgroup per example.
@@ -277,60 +293,102 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
   __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = blockDim.x, waves = threads >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int threads = blockDim.x, waves = threads >> 6;
   const int64_t b = blockIdx.x;
-  const int K = a.c.K, W = a.c.W, C = a.stretches;
+  const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
   const int64_t V = a.c.V;
-  const int64_t total = (int64_t)K * C;
-  const BmItem* item = a.item + b * total * W;
-  // (asked for before the normalisers are formed)
-  const BmItem first = tid < total ? item[(int64_t)tid * W] : BmItem{0.0f, -1};
+  const int32_t total = K * C;         // (at most 2^31 / keep, checked on the host)
+  const BmStat* stat = a.stat + b * total;
+  const BmItem* item = a.item + b * total * keep;
   if (tid == 0) s_n = 0;
   for (int k = wave; k < K; k += waves) {
     const int64_t row = b * K + k;
     double before = 0.0;
     if (a.scores) before = a.c.scores_type == CS_TYPE_F64 ? ((const double*)a.scores)[row] : (double)((const float*)a.scores)[row];
     if (a.c.normalise && !(a.finished && a.finished[row])) {
-      const BmStat* st = a.stat + row * C;
-      float m = -__builtin_inff();
-      for (int c = lane; c < C; c += 64) m = fmaxf(m, st[c].top);
-      m = bm_wave_max(m);
-      double sum = 0.0;
-      if (m > -__builtin_inff())
-        for (int c = lane; c < C; c += 64) {
-          const BmStat s = st[c];
-          // a stretch that holds NaN says so also where nothing else of it counts
-          sum += s.top > -__builtin_inff() || s.sum != s.sum ? s.sum * exp((double)fmaxf(s.top, BM_LOWEST) - (double)m) : 0.0;
-        }
-      sum = bm_wave_sum(sum);
-      before -= (double)m + log(sum);     // (+inf, NaN or nothing allowed: NaN, so that no candidate counts)
+      const BmStat* st = stat + k * C;
+      // lanes join their stretches, then each other
+      double ref = -__builtin_inf(), sum = 0.0;
+      for (int c = lane; c < C; c += 64) {
+        const BmStat s = st[c];
+        if (s.sum != s.sum) sum = s.sum;             // (NaN stays)
+        if (!(s.top > -__builtin_inff())) continue;  // nothing allowed there
+        const double m = fmax(ref, s.ref);
+        sum = sum * exp(ref - m) + s.sum * exp(s.ref - m);
+        ref = m;
+      }
+      double m = ref;
+      for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+      sum = bm_wave_sum(ref > -__builtin_inf() ? sum * exp(ref - m) : sum);
+      before -= m + log(sum);          // (+inf, NaN or nothing allowed: NaN or +inf, with no candidate left to count)
     }
     if (lane == 0) s_beam[k] = before;
   }
   __syncthreads();
-  // the W-th largest among the stretches' best bounds the result from below
-  uint64_t best = 0;
-  for (int64_t g = tid; g < total; g += threads) {
-    const BmItem i = g == tid ? first : item[g * W];
-    if (i.v >= 0) {
-      const uint64_t key = bm_key64((double)i.x + s_beam[g / C]);
+  auto key_of = [&](float x, int g) { return bm_key64((double)x + s_beam[g / C]); };
+  // a bound from below in two steps.  First the W-th largest score, as far as its leading 32 bits say, among the lanes' best
+  // of a wavefront: of the stretches' largest logits or, where these are few, of all kept ones.
+  const bool by_stretch = total >= 4 * W;
+  uint32_t best = 0;
+  if (by_stretch) {
+    for (int g = tid; g < total; g += threads) {
+      const float x = stat[g].top;
+      const uint32_t key = x > -__builtin_inff() ? (uint32_t)(key_of(x, g) >> 32) : 0u;
       best = key > best ? key : best;
     }
+  } else {
+    for (int i = tid; i < total * keep; i += threads) {
+      const int g = i / keep;
+      if (i - g * keep < stat[g].n) {
+        const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
+        best = key > best ? key : best;
+      }
+    }
   }
-  const uint64_t t_wave = bm_wave_threshold<uint64_t>(best, W);
+  const uint32_t t_wave = bm_wave_threshold<32>(best, W);
   if (lane == 0) s_wave[wave] = t_wave;
   __syncthreads();
-  uint64_t t = 1;
-  for (int w = 0; w < waves; ++w) t = s_wave[w] > t ? s_wave[w] : t;
-  for (int64_t g = tid; g < total; g += threads) {
-    const int k = (int)(g / C);
-    for (int r = 0; r < W; ++r) {          // sorted: the first that falls short ends the stretch
-      const BmItem i = item[g * W + r];
-      if (i.v < 0) break;
-      const uint64_t key = bm_key64((double)i.x + s_beam[k]);
-      if (key < t) break;
-      const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
-      if (at < cap) { s_key[at] = key; s_at[at] = k * V + i.v; }
+  uint32_t t32 = 1;
+  for (int w = 0; w < waves; ++w) t32 = s_wave[w] > t32 ? (uint32_t)s_wave[w] : t32;
+  // Then, with several wavefronts, the W-th largest of the lanes' best that are left.
+  if (waves > 1) {
+    uint32_t* s_best = (uint32_t*)s_key;           // [threads] (threads <= 2 cap)
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    if (best >= t32) s_best[atomicAdd(&s_n, 1)] = best;
+    __syncthreads();
+    const int left = s_n;
+    __syncthreads();
+    if (tid == 0) { s_n = 0; s_wave[0] = t32; }
+    __syncthreads();
+    if (left > W && tid < left) {
+      const uint32_t mine = s_best[tid];
+      int before = 0;
+      for (int j = 0; j < left; ++j) before += s_best[j] > mine || (s_best[j] == mine && j < tid);
+      if (before == W - 1) s_wave[0] = mine;
+    }
+    __syncthreads();
+    t32 = (uint32_t)s_wave[0];
+  }
+  const uint64_t t = t32 > 1 ? (uint64_t)t32 << 32 : 1;
+  auto offer = [&](const BmItem& i, int g) {
+    const uint64_t key = key_of(i.x, g);
+    if (key < t) return;
+    const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
+    if (at < cap) { s_key[at] = key; s_at[at] = (g / C) * V + i.v; }
+  };
+  // a wavefront looks at 64 stretches and then, together, through each whose largest logit reaches the bound
+  for (int g0 = wave * 64; g0 < total; g0 += threads) {
+    const int g = g0 + lane;
+    const float x = g < total ? stat[g].top : -__builtin_inff();
+    const int n_mine = g < total ? stat[g].n : 0;
+    uint64_t q = __ballot(n_mine > 0 && x > -__builtin_inff() && key_of(x, g) >= t);
+    while (q) {
+      const int s = (int)__ffsll((unsigned long long)q) - 1;
+      q &= q - 1;
+      const int n = __shfl(n_mine, s);
+      for (int r = lane; r < n; r += 64) offer(item[(int64_t)(g0 + s) * keep + r], g0 + s);
     }
   }
   __syncthreads();
@@ -360,15 +418,12 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   for (int w = 0; w < W; ++w) {
     uint64_t key = 0;
     int64_t at = 0;
-    for (int64_t g = tid; g < total; g += threads) {
-      const int k = (int)(g / C);
-      for (int r = 0; r < W; ++r) {
-        const BmItem i = item[g * W + r];
-        if (i.v < 0) break;
-        const uint64_t u = bm_key64((double)i.x + s_beam[k]);
-        const int64_t f = k * V + i.v;
-        if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
-      }
+    for (int i = tid; i < total * keep; i += threads) {
+      const int g = i / keep;
+      if (i - g * keep >= stat[g].n) continue;
+      const uint64_t u = key_of(item[i].x, g);
+      const int64_t f = (g / C) * V + item[i].v;
+      if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
     }
     for (int o = 32; o; o >>= 1) {
       const uint64_t u = __shfl_xor((unsigned long long)key, o);
@@ -382,27 +437,37 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     for (int v = 1; v < waves; ++v)
       if (s_wave[v] > key || (s_wave[v] == key && s_wave_at[v] < at)) { key = s_wave[v]; at = s_wave_at[v]; }
     if (tid == 0) put(w, key, at);
-    last = key ? key : 0;
+    last = key;
     last_at = key ? at : INT64_MAX;
   }
 }
 
+// values per lane of a stretch
+int lane_values(const cs_beam_cfg& c) { return 32; }
+int32_t stretches_of(const cs_beam_cfg& c) {
+  const int64_t len = 64 * lane_values(c);
+  return (int32_t)((c.V + len - 1) / len);
+}
+// logits kept of a stretch: what lies above the W-th largest of its lanes' best is a few more than W for W <= 32; for more, the
+// few best lanes no longer tell the best values, and the exact W are found
+int32_t keep_of(const cs_beam_cfg& c) { return c.W <= 32 ? 2 * c.W + 32 : 96; }
+
 template <typename T>
 void launch_scan(const BmArgs& a, dim3 grid, hipStream_t st) {
-  if (a.mask) hipLaunchKernelGGL((cs_beam_scan_kernel<T, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((cs_beam_scan_kernel<T, false>), grid, dim3(256), 0, st, a);
+  if (a.mask) hipLaunchKernelGGL((cs_beam_scan_kernel<T, true, 32>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((cs_beam_scan_kernel<T, false, 32>), grid, dim3(256), 0, st, a);
 }
 
 int check_beam(const cs_beam_cfg* c) {
   CS_REQUIRE(c, "null argument");
   CS_REQUIRE(c->B >= 0 && c->K >= 1 && c->K <= BM_MAXK, "1 .. 2048 beams");
-  CS_REQUIRE(c->V >= 1 && c->V <= (int64_t)INT32_MAX - 2 * BM_STRETCH, "bad number of values");
+  CS_REQUIRE(c->V >= 1 && c->V <= (int64_t)INT32_MAX - 65536, "bad number of values");
   CS_REQUIRE(c->W >= 1 && c->W <= BM_MAXW, "width must be 1 .. 64");
   CS_REQUIRE(c->logits_type == CS_TYPE_F32 || c->logits_type == CS_TYPE_BF16 || c->logits_type == CS_TYPE_F16,
              "logits are float32, bfloat16 or float16");
   CS_REQUIRE(c->scores_type == CS_TYPE_F32 || c->scores_type == CS_TYPE_F64, "scores are float32 or float64");
-  const int64_t stretches = (c->V + BM_STRETCH - 1) / BM_STRETCH;
-  CS_REQUIRE((int64_t)c->B * c->K <= ((int64_t)INT32_MAX * 4) / stretches, "too many logits for one call");
+  CS_REQUIRE((int64_t)c->K * stretches_of(*c) <= INT32_MAX / keep_of(*c) && (int64_t)c->B * c->K <= INT32_MAX / stretches_of(*c),
+             "too many logits for one call");
   return CS_OK;
 }
 
@@ -410,8 +475,7 @@ int check_beam(const cs_beam_cfg* c) {
 
 extern "C" int64_t cs_beam_select_workspace(const cs_beam_cfg* c) {
   if (check_beam(c)) return -1;
-  const int64_t stretches = (c->V + BM_STRETCH - 1) / BM_STRETCH;
-  return (int64_t)c->B * c->K * stretches * (int64_t)(sizeof(BmStat) + c->W * sizeof(BmItem));
+  return (int64_t)c->B * c->K * stretches_of(*c) * (int64_t)(sizeof(BmStat) + keep_of(*c) * sizeof(BmItem));
 }
 
 extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const void* logits, const uint8_t* mask,
@@ -426,7 +490,8 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   BmArgs a;
   a.c = *c;
   a.scores = scores; a.logits = logits; a.mask = mask; a.finished = finished;
-  a.stretches = (int32_t)((c->V + BM_STRETCH - 1) / BM_STRETCH);
+  a.stretches = stretches_of(*c);
+  a.keep = keep_of(*c);
   const int64_t items = (int64_t)c->B * c->K * a.stretches;
   a.stat = (BmStat*)workspace;
   a.item = (BmItem*)(a.stat + items);
@@ -437,12 +502,12 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, grid, st);
   else launch_scan<_Float16>(a, grid, st);
   CS_HIP(hipGetLastError());
-  // a place for W candidates of each of W stretches, up to 32 KB
-  int cap = c->W * c->W;
-  cap = cap < 256 ? 256 : cap > 2048 ? 2048 : cap;
-  // a thread per stretch, as far as that goes
-  const int64_t total = (int64_t)c->K * a.stretches;
-  const int threads = total <= 64 && c->K <= 4 ? 64 : total <= 256 ? 256 : BM_JOIN;
+  // places for what reaches the joined bound
+  const int cap = c->W * 32 < 512 ? 512 : c->W * 32 > 2048 ? 2048 : c->W * 32;
+  // a wavefront per beam and a thread per stretch, as far as that goes
+  int64_t waves = ((int64_t)c->K * a.stretches + 63) / 64;
+  waves = waves > c->K ? waves : c->K;
+  const int threads = 64 * (int)(waves < BM_JOIN / 64 ? waves : BM_JOIN / 64);
   hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads), (size_t)(((c->K * 8 + 15) & ~15) + cap * 16), st, a,
                      cap);
   CS_HIP(hipGetLastError());
