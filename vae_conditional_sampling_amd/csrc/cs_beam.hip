@@ -10,6 +10,7 @@
 // 64 bits: two beams' candidates are often closer than float32 sums of 10^5 terms are exact, and the indices are to be
 // those of the definition.
 #include "cs_common.h"
+#include "cs_div.h"
 
 namespace {
 
@@ -31,6 +32,8 @@ struct BmArgs {
   void* out_scores;
   int64_t *parents, *tokens;
   int32_t stretches, keep;
+  uint32_t items;          // B*K*stretches
+  CsDiv by_stretches, by_K, by_keep;
 };
 
 __device__ __forceinline__ uint32_t bm_key(float v) {
@@ -56,7 +59,6 @@ template <> struct BmElem<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
   }
-  static __device__ __forceinline__ float one(const float* p) { return *p; }
 };
 struct BmBf16 { uint16_t u; };
 template <> struct BmElem<BmBf16> {
@@ -68,7 +70,6 @@ template <> struct BmElem<BmBf16> {
       x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ float one(const BmBf16* p) { return __uint_as_float((uint32_t)p->u << 16); }
 };
 template <> struct BmElem<_Float16> {
   static constexpr int N = 8;
@@ -81,16 +82,28 @@ template <> struct BmElem<_Float16> {
       x[2 * i + 1] = (float)h.y;
     }
   }
-  static __device__ __forceinline__ float one(const _Float16* p) { return (float)*p; }
 };
 
+// Reductions by DPP moves within and across the rows of 16 lanes; lane 63 ends with the result of all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int bm_dpp(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+constexpr int BM_SHR = 0x110, BM_BCAST15 = 0x142, BM_BCAST31 = 0x143;
 __device__ __forceinline__ float bm_wave_max(float v) {
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
+#define CS_STEP(CTRL_, ROWS_) v = fmaxf(v, __int_as_float(bm_dpp<CTRL_, ROWS_>(__float_as_int(v), __float_as_int(v))));
+  CS_STEP(BM_SHR + 1, 0xf) CS_STEP(BM_SHR + 2, 0xf) CS_STEP(BM_SHR + 4, 0xf) CS_STEP(BM_SHR + 8, 0xf)
+  CS_STEP(BM_BCAST15, 0xa) CS_STEP(BM_BCAST31, 0xc)
+#undef CS_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 __device__ __forceinline__ double bm_wave_sum(double v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+#define CS_STEP(CTRL_, ROWS_) \
+  v += __hiloint2double(bm_dpp<CTRL_, ROWS_>(0, __double2hiint(v)), bm_dpp<CTRL_, ROWS_>(0, __double2loint(v)));
+  CS_STEP(BM_SHR + 1, 0xf) CS_STEP(BM_SHR + 2, 0xf) CS_STEP(BM_SHR + 4, 0xf) CS_STEP(BM_SHR + 8, 0xf)
+  CS_STEP(BM_BCAST15, 0xa) CS_STEP(BM_BCAST31, 0xc)
+#undef CS_STEP
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
 }
 
 // 2^(j / 64)
@@ -112,16 +125,16 @@ __device__ const double bm_pow64[64] = {
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509};
 
-// exp(d) 2^-n0 as 2^(n - n0) 2^(j/64) exp(r), 64 n + j the integer nearest to 64 d / ln 2 and |r| <= ln 2 / 128, exp(r) by its
+// exp(d) for |d| <= 690 as 2^n 2^(j/64) exp(r), 64 n + j the integer nearest to 64 d / ln 2 and |r| <= ln 2 / 128, exp(r) by its
 // Taylor polynomial of degree 3 (remainder r^4 / 24 < 3.6e-11): the table-driven method of Tang (1989).  Adding 1.5 * 2^52
 // leaves the integer in the low word.  The table lies in the lanes' registers and is read by ds_bpermute, which takes the
-// lane from the index's low 6 bits by itself; its high words have j << 14 and n0 << 20 taken off beforehand, so one shift and
-// addition of the whole integer puts the exponent right.
+// lane from the index's low 6 bits by itself; its high words have j << 14 taken off beforehand, so one shift and addition of
+// the whole integer puts the exponent right.
 struct BmPow {
   int hi, lo;
-  __device__ __forceinline__ BmPow(int lane, int n0) {
+  __device__ __forceinline__ explicit BmPow(int lane) {
     const double t = bm_pow64[lane];
-    hi = __double2hiint(t) - (lane << 14) - (n0 << 20);
+    hi = __double2hiint(t) - (lane << 14);
     lo = __double2loint(t);
   }
 };
@@ -154,15 +167,14 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   constexpr int N = BmElem<T>::N;      // logits in 16 bytes
   constexpr float INF = __builtin_inff();
   const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t rows = (int64_t)a.c.B * a.c.K;
-  if (item >= rows * a.stretches) return;
-  const int64_t row = item / a.stretches;
+  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= a.items) return;
+  const uint32_t row = cs_div(item, a.by_stretches);
   const int32_t base = (int32_t)(item - row * a.stretches) * (64 * LANE);
-  const int64_t b = row / a.c.K, k = row - b * a.c.K;
+  const uint32_t b = cs_div(row, a.by_K), k = row - b * a.c.K;
   const int W = a.c.W, keep = a.keep;
   const int32_t V = (int32_t)a.c.V;
-  BmItem* out = a.item + item * keep;
+  BmItem* out = a.item + (int64_t)item * keep;
   if (a.finished && a.finished[row]) {   // its one candidate keeps the beam's score; its logits are not read
     if (lane == 0) {
       a.stat[item] = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
@@ -172,56 +184,92 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   }
   const T* p = (const T*)a.logits + b * a.c.logits_stride[0] + k * a.c.logits_stride[1];
   const uint8_t* mk = MASK ? a.mask + b * a.c.mask_stride[0] + k * a.c.mask_stride[1] : nullptr;
+  constexpr int VECS = LANE / N;
   float x[LANE];
+  float best = -INF, least = INF;      // (a NaN is passed over)
+  double ref = 0.0, sum = 0.0, sum1 = 0.0;
+  const BmPow pow(lane);
+  uint32_t raw[VECS][4];
+  if (!MASK && base + 64 * LANE <= V) {
 #pragma unroll
-  for (int j = 0; j < LANE / N; ++j) {
-    const int32_t v0 = base + (j * 64 + lane) * N;
-    if (v0 + N <= V) {
-      uint32_t r[4];
-      __builtin_memcpy(r, p + v0, 16);
-      BmElem<T>::widen(r, x + j * N);
-      if (MASK) {
-        uint8_t m[N];
-        __builtin_memcpy(m, mk + v0, N);
+    for (int j = 0; j < VECS; ++j) __builtin_memcpy(raw[j], p + base + (j * 64 + lane) * N, 16);
+    // the sum is formed as the values come in, as if none of them were beyond 690; that is seen to below
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[j * N + e] = m[e] ? x[j * N + e] : -INF;
+    for (int j = 0; j < VECS; ++j) {
+      BmElem<T>::widen(raw[j], x + j * N);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        best = fmaxf(best, x[j * N + e]);
+        least = fminf(least, x[j * N + e]);
       }
-    } else {
+      if (a.c.normalise) {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        x[j * N + e] = v0 + e < V && (!MASK || mk[v0 + e]) ? BmElem<T>::one(p + v0 + e) : -INF;
+        for (int e = 0; e < N; e += 2) {
+          sum = bm_add_exp(sum, (double)x[j * N + e], pow);
+          sum1 = bm_add_exp(sum1, (double)x[j * N + e + 1], pow);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  } else {
+    // the same where values are not allowed or lie beyond the row's end: -690 in the sum and -inf as a candidate
+    uint8_t m[VECS][N];
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      const int32_t v0 = base + (j * 64 + lane) * N;
+      if (v0 + N <= V) {
+        __builtin_memcpy(raw[j], p + v0, 16);
+        if (MASK) __builtin_memcpy(m[j], mk + v0, N);
+      } else {
+        T one[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int32_t v = v0 + e < V ? v0 + e : V - 1;
+          one[e] = p[v];
+          if (MASK) m[j][e] = mk[v];
+        }
+        __builtin_memcpy(raw[j], one, 16);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      BmElem<T>::widen(raw[j], x + j * N);
+      float y[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const bool there = base + (j * 64 + lane) * N + e < V && (!MASK || m[j][e]);
+        y[e] = there ? x[j * N + e] : -690.0f;
+        x[j * N + e] = there ? x[j * N + e] : -INF;
+        best = fmaxf(best, x[j * N + e]);
+        least = fminf(least, y[e]);
+      }
+      if (a.c.normalise) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          sum = bm_add_exp(sum, (double)y[e], pow);
+          sum1 = bm_add_exp(sum1, (double)y[e + 1], pow);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
-  float best = -INF, least = INF;      // (a NaN is passed over)
-#pragma unroll
-  for (int i = 0; i < LANE; ++i) {
-    best = fmaxf(best, x[i]);
-    least = fminf(least, x[i]);
-  }
   const float top = bm_wave_max(best);
-  double ref = 0.0, sum = 0.0, sum1 = 0.0;
   if (a.c.normalise) {
-    least = -bm_wave_max(-least);
-    if (top < 8192.0f && least > -8192.0f && top - least < 600.0f) {
-      // no exponent can leave its range (a NaN makes the sum one)
-      const int n0 = (int)__builtin_rintf(top * 1.44269504f);
-      const BmPow pow(lane, n0);
-      ref = n0 * 0.6931471805599453;
-#pragma unroll
-      for (int i = 0; i < LANE; i += 2) {
-        sum = bm_add_exp(sum, (double)x[i], pow);
-        sum1 = bm_add_exp(sum1, (double)x[i + 1], pow);
-      }
-    } else {
+    if (top < -600.0f || top > 690.0f || __ballot(least < -690.0f)) {
       bool nan = false;
+      sum = sum1 = 0.0;
 #pragma unroll
       for (int i = 0; i < LANE; ++i) nan = nan || x[i] != x[i];
       if (top > -INF) {
-        const BmPow pow(lane, 0);
         ref = (double)top;
         // (less than exp(-690) counts as that; of an infinite top every difference is NaN or -inf)
 #pragma unroll
-        for (int i = 0; i < LANE; ++i) sum = bm_add_exp(sum, fmax((double)x[i] - ref, -690.0), pow);
+        for (int i = 0; i < LANE; ++i) {
+          float xi = x[i];
+          asm("" : "+v"(xi));   // (else the conversions of both branches are made above them and kept: 64 more registers)
+          sum = bm_add_exp(sum, fmax((double)xi - ref, -690.0), pow);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if (__ballot(nan) || top == INF) sum = __builtin_nan("");
     }
@@ -236,7 +284,7 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   for (int i = 0; i < LANE; ++i) {
     const uint64_t m = __ballot(x[i] >= t);
     if (m) {
-      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
       n += __popcll(m);
       if (n <= keep && x[i] >= t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
     }
@@ -326,7 +374,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     if (lane == 0) s_beam[k] = before;
   }
   __syncthreads();
-  auto key_of = [&](float x, int g) { return bm_key64((double)x + s_beam[g / C]); };
+  auto key_of = [&](float x, int g) { return bm_key64((double)x + s_beam[cs_div(g, a.by_stretches)]); };
   // a bound from below in two steps.  First the W-th largest score, as far as its leading 32 bits say, among the lanes' best
   // of a wavefront: of the stretches' largest logits or, where these are few, of all kept ones.
   const bool by_stretch = total >= 4 * W;
@@ -339,7 +387,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     }
   } else {
     for (int i = tid; i < total * keep; i += threads) {
-      const int g = i / keep;
+      const int g = cs_div(i, a.by_keep);
       if (i - g * keep < stat[g].n) {
         const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
         best = key > best ? key : best;
@@ -376,7 +424,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     const uint64_t key = key_of(i.x, g);
     if (key < t) return;
     const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
-    if (at < cap) { s_key[at] = key; s_at[at] = (g / C) * V + i.v; }
+    if (at < cap) { s_key[at] = key; s_at[at] = (int64_t)cs_div(g, a.by_stretches) * V + i.v; }
   };
   // a wavefront looks at 64 stretches and then, together, through each whose largest logit reaches the bound
   for (int g0 = wave * 64; g0 < total; g0 += threads) {
@@ -419,10 +467,10 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     uint64_t key = 0;
     int64_t at = 0;
     for (int i = tid; i < total * keep; i += threads) {
-      const int g = i / keep;
+      const int g = cs_div(i, a.by_keep);
       if (i - g * keep >= stat[g].n) continue;
       const uint64_t u = key_of(item[i].x, g);
-      const int64_t f = (g / C) * V + item[i].v;
+      const int64_t f = (int64_t)cs_div(g, a.by_stretches) * V + item[i].v;
       if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
     }
     for (int o = 32; o; o >>= 1) {
@@ -442,8 +490,12 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   }
 }
 
-// values per lane of a stretch
-int lane_values(const cs_beam_cfg& c) { return 32; }
+// values per lane of a stretch: 32 where that fills the chip (6 wavefronts on each of its 1024 SIMDs), else 16 or 8
+int lane_values(const cs_beam_cfg& c) {
+  int lane = 32;
+  while (lane > 8 && (int64_t)c.B * c.K * ((c.V + 64 * lane - 1) / (64 * lane)) < 6144) lane /= 2;
+  return lane;
+}
 int32_t stretches_of(const cs_beam_cfg& c) {
   const int64_t len = 64 * lane_values(c);
   return (int32_t)((c.V + len - 1) / len);
@@ -454,8 +506,15 @@ int32_t keep_of(const cs_beam_cfg& c) { return c.W <= 32 ? 2 * c.W + 32 : 96; }
 
 template <typename T>
 void launch_scan(const BmArgs& a, dim3 grid, hipStream_t st) {
-  if (a.mask) hipLaunchKernelGGL((cs_beam_scan_kernel<T, true, 32>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((cs_beam_scan_kernel<T, false, 32>), grid, dim3(256), 0, st, a);
+  switch (lane_values(a.c)) {
+#define CS_SCAN(L_)                                                                                              \
+    case L_:                                                                                                     \
+      if (a.mask) hipLaunchKernelGGL((cs_beam_scan_kernel<T, true, L_>), grid, dim3(256), 0, st, a);             \
+      else hipLaunchKernelGGL((cs_beam_scan_kernel<T, false, L_>), grid, dim3(256), 0, st, a);                   \
+      break;
+    CS_SCAN(8) CS_SCAN(16) CS_SCAN(32)
+#undef CS_SCAN
+  }
 }
 
 int check_beam(const cs_beam_cfg* c) {
@@ -497,6 +556,10 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   a.item = (BmItem*)(a.stat + items);
   a.out_scores = out_scores; a.parents = parents; a.tokens = tokens;
   hipStream_t st = (hipStream_t)stream;
+  a.items = (uint32_t)items;
+  a.by_stretches = cs_div_by(a.stretches);
+  a.by_K = cs_div_by(c->K);
+  a.by_keep = cs_div_by(a.keep);
   const dim3 grid((unsigned)((items + 3) / 4));
   if (c->logits_type == CS_TYPE_F32) launch_scan<float>(a, grid, st);
   else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, grid, st);

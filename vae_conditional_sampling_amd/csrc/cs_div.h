@@ -1,0 +1,19 @@
+// n / d for any 32-bit n by a multiplication (the round-up form of Granlund and Montgomery, 1994), d from 1 to 2^32 - 1: a
+// 64-bit division by a size of the call costs a lane several hundred instructions, a 32-bit one about forty.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+struct CsDiv {
+  uint32_t d, mul, shift;
+};
+inline CsDiv cs_div_by(int64_t d) {
+  uint32_t l = 0;
+  while (l < 32 && (1ull << l) < (uint64_t)d) ++l;
+  const uint64_t mul = ((1ull << 32) * ((1ull << l) - (uint64_t)d)) / (uint64_t)d + 1;
+  return CsDiv{(uint32_t)d, (uint32_t)mul, l};
+}
+__device__ __forceinline__ uint32_t cs_div(uint32_t n, const CsDiv& d) {
+  const uint32_t t = __umulhi(n, d.mul);
+  return d.shift == 0 ? n : (t + ((n - t) >> 1)) >> (d.shift - 1);
+}

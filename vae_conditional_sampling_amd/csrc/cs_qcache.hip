@@ -12,26 +12,11 @@
 //          scale becomes 255 and the group reads as NaN.
 // A lane holds 8 values, G / 8 neighbouring lanes share a group's maximum; both directions are bound by memory.
 #include "cs_common.h"
+#include "cs_div.h"
 
 namespace {
 
 constexpr int QC_LANE = 8;     // values a lane holds
-
-// n / d and n mod d for any 32-bit n by a multiplication (Granlund and Montgomery's round-up form): 64-bit divisions by
-// the sizes of a call cost several hundred instructions per lane, more than all else these kernels do.
-struct QcDiv {
-  uint32_t d, mul, shift;
-};
-QcDiv qc_div(int64_t d) {
-  uint32_t l = 0;
-  while (l < 32 && (1ull << l) < (uint64_t)d) ++l;
-  const uint64_t mul = ((1ull << 32) * ((1ull << l) - (uint64_t)d)) / (uint64_t)d + 1;
-  return QcDiv{(uint32_t)d, (uint32_t)mul, l};
-}
-__device__ __forceinline__ uint32_t qc_over(uint32_t n, const QcDiv& d) {
-  const uint32_t t = __umulhi(n, d.mul);
-  return d.shift == 0 ? n : (t + ((n - t) >> 1)) >> (d.shift - 1);
-}
 
 struct QcArgs {
   cs_qcache c;
@@ -40,7 +25,7 @@ struct QcArgs {
   int32_t lanes;               // lanes of a row: groups * G / 8
   int32_t rows_per_block;
   uint32_t rows;               // rows of the call, below 2^31
-  QcDiv by_lanes, by_chains, by_inner, by_T;   // lanes; B * K (write) or B * J (read); K or J; T
+  CsDiv by_lanes, by_chains, by_inner, by_T;   // lanes; B * K (write) or B * J (read); K or J; T
   const void* x;               // write
   void* out;                   // read
   int64_t stride[3];
@@ -155,7 +140,7 @@ __device__ __forceinline__ int32_t qc_slot(const QcArgs& a, uint32_t i, uint32_t
     if (far < 0) return -1;
     s = far < (int64_t)T ? (uint32_t)far : (uint32_t)(far % (int64_t)T);
   }
-  s += i - qc_over(i, a.by_T) * T;
+  s += i - cs_div(i, a.by_T) * T;
   return (int32_t)(s >= T ? s - T : s);
 }
 
@@ -177,12 +162,12 @@ __device__ __forceinline__ void qc_store8(T* p, const float* v) {
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
-  const int ry = (int)qc_over(threadIdx.x, a.by_lanes);
+  const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
   const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
   const bool live = ry < a.rows_per_block && row < a.rows;
-  const uint32_t i = live ? qc_over(row, a.by_chains) : 0, chain = live ? row - i * a.by_chains.d : 0;
+  const uint32_t i = live ? cs_div(row, a.by_chains) : 0, chain = live ? row - i * a.by_chains.d : 0;
   const int32_t slot = live ? qc_slot(a, i, chain) : -1;
-  const uint32_t b = qc_over(chain, a.by_inner), k = chain - b * a.by_inner.d;
+  const uint32_t b = cs_div(chain, a.by_inner), k = chain - b * a.by_inner.d;
   const T* x = (const T*)a.x + i * a.stride[0] + b * a.stride[1] + k * a.stride[2];
   char* rec = (char*)a.c.data + ((int64_t)(slot < 0 ? 0 : slot) * a.by_chains.d + chain) * a.record;
   const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
@@ -226,11 +211,11 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
-  const int ry = (int)qc_over(threadIdx.x, a.by_lanes);
+  const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
   const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
   if (ry >= a.rows_per_block || row >= a.rows) return;
-  const uint32_t i = qc_over(row, a.by_chains), chain = row - i * a.by_chains.d;
-  const uint32_t b = qc_over(chain, a.by_inner), j = chain - b * a.by_inner.d;
+  const uint32_t i = cs_div(row, a.by_chains), chain = row - i * a.by_chains.d;
+  const uint32_t b = cs_div(chain, a.by_inner), j = chain - b * a.by_inner.d;
   const int64_t slot = a.slots ? a.slots[row] : qc_slot(a, i, chain);
   const int64_t k = a.from ? a.from[row] : j;
   const bool there = slot >= 0 && slot < a.c.T && k >= 0 && k < a.c.K;
@@ -293,16 +278,16 @@ int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStr
   const cs_qcache& c = a.c;
   CS_REQUIRE(c.B <= INT32_MAX / inner && n <= INT32_MAX / (c.B * inner), "2^31 states or more in one call");
   a.rows = (uint32_t)(n * c.B * inner);
-  a.by_chains = qc_div(c.B * inner);
-  a.by_inner = qc_div(inner);
-  a.by_T = qc_div(c.T);
+  a.by_chains = cs_div_by(c.B * inner);
+  a.by_inner = cs_div_by(inner);
+  a.by_T = cs_div_by(c.T);
   a.start0 = start0 % c.T;
   CS_REQUIRE(type == CS_TYPE_F32 || type == CS_TYPE_BF16 || type == CS_TYPE_F16, "states are float32, bfloat16 or float16");
   CS_REQUIRE(((uintptr_t)c.data & 15) == 0, "the ring must be 16-byte aligned");
   a.record = cs_qcache_record_bytes(c.fmt, c.group, c.D);
   a.code_bytes = (int32_t)code_bytes_of(c.fmt, c.D);
   a.lanes = (c.D + c.group - 1) / c.group * (c.group / QC_LANE);
-  a.by_lanes = qc_div(a.lanes);
+  a.by_lanes = cs_div_by(a.lanes);
   a.rows_per_block = a.lanes >= 256 ? 1 : 256 / a.lanes;
   const dim3 grid((a.rows + a.rows_per_block - 1) / a.rows_per_block);
   if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, grid, st);
