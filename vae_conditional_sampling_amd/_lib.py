@@ -291,29 +291,29 @@ def ptr(t):
     return t.data_ptr()
 
 
-def on_device(*tensors):
-    """The CUDA device of all given tensors (None is passed over), for entry points that also serve tensors of another
-    device than the current one."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise CsError("libcsvae operates on device tensors only (no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise CsError(f"tensors on different devices: {dev} and {t.device}")
+def on_device(t, *others):
+    """The device of CUDA tensor ``t`` and of all ``others`` (None is passed over), for entry points that also serve tensors of
+    another device than the current one."""
+    dev = t.device
+    for o in (t, *others):
+        if o is not None and (not o.is_cuda or o.device != dev):
+            if not o.is_cuda:
+                raise CsError("libcsvae operates on device tensors only (no CPU path)")
+            raise CsError(f"tensors on different devices: {dev} and {o.device}")
     return dev
 
 
 def call_on(dev, fn, *args):
     """``check(fn(*args, stream))`` on the current stream of ``dev``, with ``dev`` current for the call."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    index = dev.index
+    # (the stream's handle itself: making torch's stream object costs as much as a launch)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def make_rng(seed, iteration=0, example_offset=0):

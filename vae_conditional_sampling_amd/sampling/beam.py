@@ -6,6 +6,7 @@ The beams of an example are its chains ``[B,K]``; every beam can continue with `
 history in 8 or 4 bits and reorders it likewise.  The reference has no counterpart.
 """
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -21,13 +22,24 @@ class BeamStep(NamedTuple):
     tokens: torch.Tensor    # [B,W] int64: the value it continues with
 
 
-def _flags(t, what, dev):
+def _flags(t, what):
     """uint8 view of a bool / uint8 tensor."""
     if t.dtype == torch.bool:
-        t = t.view(torch.uint8)
-    elif t.dtype != torch.uint8:
+        return t.view(torch.uint8)
+    if t.dtype != torch.uint8:
         raise _lib.CsError(f"{what} must be a bool or uint8 tensor, got {t.dtype}")
     return t
+
+
+@functools.lru_cache(maxsize=256)
+def _select_cfg(B, K, V, width, logits_type, scores_type, normalise, end_token, ls0, ls1, ms0, ms1):
+    """(cs_beam_cfg, bytes of workspace) of calls of one shape; read only."""
+    pair = C.c_int64 * 2
+    cfg = _lib.cs_beam_cfg(B, K, V, width, logits_type, scores_type, normalise, end_token, pair(ls0, ls1), pair(ms0, ms1))
+    nbytes = _lib.lib().cs_beam_select_workspace(C.byref(cfg))
+    if nbytes < 0:
+        raise _lib.CsError(f"libcsvae error: {_lib.lib().cs_last_error().decode()}")
+    return cfg, nbytes
 
 
 def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int, *, normalise: bool = True,
@@ -48,61 +60,63 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
         raise _lib.CsError(f"logits must be [B,K,V], got {tuple(logits.shape)}")
     B, K, V = logits.shape
     dev = _lib.on_device(logits, scores, mask, finished)
-    if logits.dtype not in _lib.CS_TYPE or logits.dtype == torch.float64:
+    logits_type = _lib.CS_TYPE.get(logits.dtype, 3)
+    if logits_type == 3:
         raise _lib.CsError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if scores is None:
-        out_type = torch.float32
-    else:
+    out_type, scores_at, mask_at, finished_at = torch.float32, None, None, None
+    if scores is not None:
         out_type = scores.dtype
         if out_type not in (torch.float32, torch.float64):
             raise _lib.CsError(f"scores must be float32 or float64, got {out_type}")
         if scores.shape != (B, K):
             raise _lib.CsError(f"scores must be [{B},{K}], got {tuple(scores.shape)}")
         scores = scores.contiguous()
-    if logits.stride(2) != 1 and V > 1:
+        scores_at = scores.data_ptr()
+    ls = logits.stride()
+    if ls[2] != 1 and V > 1:
         logits = logits.contiguous()
-    cfg = _lib.cs_beam_cfg(B, K, V, int(width), _lib.CS_TYPE[logits.dtype], _lib.CS_TYPE[out_type], int(normalise), 0)
-    cfg.logits_stride[:] = logits.stride()[:2]
+        ls = logits.stride()
+    ms = (0, 0)
     if mask is not None:
-        mask = _flags(mask, "mask", dev).expand(B, K, V)
+        mask = _flags(mask, "mask").expand(B, K, V)
         if mask.stride(2) != 1 and V > 1:
             mask = mask.contiguous()
-        cfg.mask_stride[:] = mask.stride()[:2]
-    if finished is not None:
+        ms = mask.stride()
+        mask_at = mask.data_ptr()
+    if finished is None:
+        end_token = 0
+    else:
         if end_token is None:
             raise _lib.CsError("finished needs end_token")
-        finished = _flags(finished, "finished", dev)
+        finished = _flags(finished, "finished")
         if finished.shape != (B, K):
             raise _lib.CsError(f"finished must be [{B},{K}], got {tuple(finished.shape)}")
         finished = finished.contiguous()
-        cfg.end_token = int(end_token)
-    L = _lib.lib()
-    nbytes = L.cs_beam_select_workspace(C.byref(cfg))
-    if nbytes < 0:
-        raise _lib.CsError(f"libcsvae error: {L.cs_last_error().decode()}")
-    W = cfg.W
+        finished_at = finished.data_ptr()
+    width = int(width)
+    cfg, nbytes = _select_cfg(B, K, V, width, logits_type, _lib.CS_TYPE[out_type], int(bool(normalise)), int(end_token), ls[0],
+                              ls[1], ms[0], ms[1])
     # the workspace is the call's own (calls on several streams and captured ones share nothing)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    new_scores = torch.empty(B, W, dtype=out_type, device=dev)
-    chosen = torch.empty(2, B, W, dtype=torch.int64, device=dev)
-    parents, tokens = chosen[0], chosen[1]
-    p = lambda t: None if t is None else t.data_ptr()
-    _lib.call_on(dev, L.cs_beam_select, C.byref(cfg), p(scores), logits.data_ptr(), p(mask), p(finished),
+    new_scores = torch.empty((B, width), dtype=out_type, device=dev)
+    parents = torch.empty((B, width), dtype=torch.int64, device=dev)
+    tokens = torch.empty_like(parents)
+    _lib.call_on(dev, _lib.lib().cs_beam_select, C.byref(cfg), scores_at, logits.data_ptr(), mask_at, finished_at,
                  new_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr(), nbytes)
     return BeamStep(new_scores, parents, tokens)
 
 
-def _rows(t, axis):
-    """(outer, strides in bytes of (outer, example, chain), bytes of a row) of t[outer..., B, K, row...], or None if the
-    outer axes do not collapse into one stride or a row is not adjacent in memory."""
-    size = t.element_size()
+@functools.lru_cache(maxsize=256)
+def _rows(shape, strides, size, axis):
+    """(outer, strides in bytes of (outer, example, chain), bytes of a row) of a tensor [outer..., B, K, row...], or None if
+    the outer axes do not collapse into one stride or a row is not adjacent in memory."""
     row = 1
-    for n, s in zip(reversed(t.shape[axis + 2:]), reversed(t.stride()[axis + 2:])):
+    for n, s in zip(reversed(shape[axis + 2:]), reversed(strides[axis + 2:])):
         if n != 1 and s != row:
             return None
         row *= n
     outer, stride = 1, 0
-    for n, s in zip(reversed(t.shape[:axis]), reversed(t.stride()[:axis])):
+    for n, s in zip(reversed(shape[:axis]), reversed(strides[:axis])):
         if n == 1:
             continue
         if outer == 1:
@@ -110,7 +124,7 @@ def _rows(t, axis):
         elif s != stride * outer:
             return None
         outer *= n
-    return outer, (stride * size, t.stride(axis) * size, t.stride(axis + 1) * size), row * size
+    return outer, (C.c_int64 * 3)(stride * size, strides[axis] * size, strides[axis + 1] * size), row * size
 
 
 def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: int = 0,
@@ -126,28 +140,30 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: in
         batch_dim += states.dim()
     if not 0 <= batch_dim <= states.dim() - 2:
         raise _lib.CsError("states need an example and a chain axis")
-    B, K = states.shape[batch_dim:batch_dim + 2]
+    shape = tuple(states.shape)
+    B, K = shape[batch_dim:batch_dim + 2]
     if parents.dim() != 2 or parents.shape[0] != B or parents.dtype != torch.int64:
         raise _lib.CsError(f"parents must be int64 [{B},W], got {parents.dtype} {tuple(parents.shape)}")
     W = parents.shape[1]
-    shape = states.shape[:batch_dim + 1] + (W,) + states.shape[batch_dim + 2:]
+    out_shape = shape if W == K else shape[:batch_dim + 1] + (W,) + shape[batch_dim + 2:]
     if out is None:
-        out = torch.zeros(shape, dtype=states.dtype, device=states.device)
-    elif out.shape != shape or out.dtype != states.dtype:
-        raise _lib.CsError(f"out must be {states.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+        out = torch.zeros(out_shape, dtype=states.dtype, device=states.device)
+    elif tuple(out.shape) != out_shape or out.dtype != states.dtype:
+        raise _lib.CsError(f"out must be {states.dtype} {out_shape}, got {out.dtype} {tuple(out.shape)}")
     dev = _lib.on_device(states, parents, out)
     if out.numel() == 0:
         return out
     if K == 0:
         raise _lib.CsError("no chains")
-    src, dst = _rows(states, batch_dim), _rows(out, batch_dim)
+    size = states.element_size()
+    dst = _rows(out_shape, out.stride(), size, batch_dim)
     if dst is None:
         raise _lib.CsError("out: rows must be adjacent in memory and the leading axes of one stride")
+    src = dst if out is states else _rows(shape, states.stride(), size, batch_dim)
     if src is None:   # (never in place: out has the same layout)
         states = states.contiguous()
-        src = _rows(states, batch_dim)
+        src = _rows(shape, states.stride(), size, batch_dim)
     parents = parents.contiguous()
-    i64x3 = C.c_int64 * 3
-    _lib.call_on(dev, _lib.lib().cs_beam_reorder, states.data_ptr(), out.data_ptr(), src[0], B, K, W, src[2],
-                 i64x3(*src[1]), i64x3(*dst[1]), parents.data_ptr())
+    _lib.call_on(dev, _lib.lib().cs_beam_reorder, states.data_ptr(), out.data_ptr(), src[0], B, K, W, src[2], src[1], dst[1],
+                 parents.data_ptr())
     return out

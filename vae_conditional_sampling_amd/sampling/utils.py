@@ -152,6 +152,9 @@ class ImputationHistoryQueue_with_restrictedavailability(object):
         return r
 
 
+_STRIDES = C.c_int64 * 3
+
+
 class QuantisedHistory:
     """Ring ``[T,B,K,D]`` of past states in 8 or 4 bits: quantised as they are written, read back by slot and chain.
 
@@ -170,20 +173,23 @@ class QuantisedHistory:
         self.record_bytes = int(_lib.lib().cs_qcache_record_bytes(_lib.CS_QFMT[fmt], group, D))
         if self.record_bytes < 0 or self.max_history_length < 1 or K < 1:
             raise _lib.CsError(f"no history of {self.max_history_length} states {self.batch_shape} as {fmt}, groups of {group}")
-        self.data = torch.zeros((self.max_history_length, B, K, self.record_bytes), dtype=torch.uint8, device=device)
         self._desc = _lib.cs_qcache(None, self.max_history_length, B, K, D, _lib.CS_QFMT[fmt], group)
+        self._ring = C.byref(self._desc)
+        self.data = torch.zeros((self.max_history_length, B, K, self.record_bytes), dtype=torch.uint8, device=device)
 
-    def _ring(self):
-        """The C description of the ring as it is now (``data`` may have been moved or replaced by one of its shape)."""
-        d = self.data
-        if d.shape != (self.max_history_length,) + self.batch_shape[:2] + (self.record_bytes,) or d.dtype != torch.uint8 \
-                or not d.is_contiguous():
-            raise _lib.CsError("data must stay a contiguous uint8 [T,B,K,record]")
-        self._desc.data = d.data_ptr()
-        return C.byref(self._desc)
+    @property
+    def data(self):
+        return self._data
+
+    @data.setter
+    def data(self, t):
+        if tuple(t.shape) != (self.max_history_length,) + self.batch_shape[:2] + (self.record_bytes,) or t.dtype != torch.uint8 \
+                or not t.is_contiguous() or t.data_ptr() % 16:
+            raise _lib.CsError("data must be a contiguous uint8 [T,B,K,record], aligned to 16 bytes")
+        self._data, self._desc.data = t, t.data_ptr()
 
     def _int64(self, t, shape, what):
-        if t.dtype != torch.int64 or tuple(t.shape) != shape:
+        if t.dtype != torch.int64 or t.shape != shape:
             raise _lib.CsError(f"{what} must be int64 {list(shape)}, got {t.dtype} {list(t.shape)}")
         return t.contiguous()
 
@@ -193,71 +199,76 @@ class QuantisedHistory:
         the chain is left out).  ``counts`` (int64 [B,K]): only the first ``counts[b,k]`` states of a chain are written; all
         other records stay as they are."""
         B, K, D = self.batch_shape
-        if X.dim() == 3:
-            X = X[None]
-        if X.dim() != 4 or tuple(X.shape[1:]) != (B, K, D):
-            raise _lib.CsError(f"states must be [n,{B},{K},{D}], got {list(X.shape)}")
-        if X.dtype not in _lib.CS_TYPE or X.dtype == torch.float64:
+        shape = X.shape
+        if shape[-3:] != self.batch_shape or len(shape) not in (3, 4):
+            raise _lib.CsError(f"states must be [n,{B},{K},{D}], got {list(shape)}")
+        kind = _lib.CS_TYPE.get(X.dtype, 3)
+        if kind == 3:
             raise _lib.CsError(f"states must be float32, bfloat16 or float16, got {X.dtype}")
-        tensor = torch.is_tensor(start)
-        dev = _lib.on_device(self.data, X, start if tensor else None, counts)
-        if X.stride(3) != 1 and D > 1:
-            X = X.contiguous()
-        if tensor:
+        start_at, first, counts_at = None, 0, None
+        if torch.is_tensor(start):
             start = self._int64(start, (B, K), "start")
+            start_at = start.data_ptr()
+        else:
+            first = int(start)
         if counts is not None:
             counts = self._int64(counts, (B, K), "counts")
-        _lib.call_on(dev, _lib.lib().cs_qcache_write, self._ring(), X.data_ptr(), _lib.CS_TYPE[X.dtype], X.shape[0],
-                     (C.c_int64 * 3)(*X.stride()[:3]), start.data_ptr() if tensor else None, 0 if tensor else int(start),
-                     None if counts is None else counts.data_ptr())
+            counts_at = counts.data_ptr()
+        dev = _lib.on_device(self._data, X, start if start_at else None, counts)
+        strides = X.stride()
+        if strides[-1] != 1 and D > 1:
+            X = X.contiguous()
+            strides = X.stride()
+        _lib.call_on(dev, _lib.lib().cs_qcache_write, self._ring, X.data_ptr(), kind, shape[0] if len(shape) == 4 else 1,
+                     _STRIDES(*(strides[:3] if len(shape) == 4 else (0, strides[0], strides[1]))), start_at, first, counts_at)
 
     def read(self, slots, chains=None, *, dtype=torch.float32, out=None):
         """``out[n,b,j] = state at slots[n,b,j] of chain chains[n,b,j]`` (None: of chain j) of example b, zeros where slot or
         chain do not exist.  ``slots`` / ``chains`` int64 [N,B,J] or [B,J]; ``out`` [N,B,J,D] (or [B,J,D]): any strides with D
         adjacent."""
         B, K, D = self.batch_shape
-        single = slots.dim() == 2
-        if single:
-            slots = slots[None]
-            chains = None if chains is None else chains[None]
-            out = None if out is None else out[None]
-        if slots.dim() != 3 or slots.shape[1] != B or slots.dtype != torch.int64 or (chains is None and slots.shape[2] != K):
-            raise _lib.CsError(f"slots must be int64 [N,{B},{K}] (or [N,{B},J] with chains), got {slots.dtype} {list(slots.shape)}")
-        N, _, J = slots.shape
+        shape = tuple(slots.shape)
+        if len(shape) not in (2, 3) or shape[-2] != B or slots.dtype != torch.int64 or (chains is None and shape[-1] != K):
+            raise _lib.CsError(f"slots must be int64 [N,{B},{K}] (or [N,{B},J] with chains), got {slots.dtype} {list(shape)}")
+        chains_at = None
         if chains is not None:
-            chains = self._int64(chains, (N, B, J), "chains")
+            chains = self._int64(chains, shape, "chains")
+            chains_at = chains.data_ptr()
         slots = slots.contiguous()
-        out = self._out(out, (N, B, J, D), dtype)
+        out, kind, strides = self._out(out, shape + (D,), dtype)
         if out.numel():
-            dev = _lib.on_device(self.data, slots, chains, out)
-            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring(), slots.data_ptr(), 0,
-                         None if chains is None else chains.data_ptr(), N, J, out.data_ptr(), _lib.CS_TYPE[out.dtype],
-                         (C.c_int64 * 3)(*out.stride()[:3]))
-        return out[0] if single else out
+            dev = _lib.on_device(self._data, slots, chains, out)
+            single = len(shape) == 2
+            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring, slots.data_ptr(), 0, chains_at, 1 if single else shape[0],
+                         shape[-1], out.data_ptr(), kind, _STRIDES(*((0,) + strides[:2] if single else strides[:3])))
+        return out
 
     def read_steps(self, start, n, *, dtype=torch.float32, out=None):
         """The states of all chains at the slots ``start .. start + n - 1`` (mod T): [n,B,K,D]."""
         B, K, D = self.batch_shape
-        out = self._out(out, (int(n), B, K, D), dtype)
+        out, kind, strides = self._out(out, (int(n), B, K, D), dtype)
         if out.numel():
-            dev = _lib.on_device(self.data, out)
-            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring(), None, int(start), None, int(n), K, out.data_ptr(),
-                         _lib.CS_TYPE[out.dtype], (C.c_int64 * 3)(*out.stride()[:3]))
+            dev = _lib.on_device(self._data, out)
+            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring, None, int(start), None, int(n), K, out.data_ptr(), kind,
+                         _STRIDES(*strides[:3]))
         return out
 
     def _out(self, out, shape, dtype):
+        """(the tensor to read into, its element type, its strides)"""
         if out is None:
-            if dtype not in _lib.CS_TYPE or dtype == torch.float64:
+            kind = _lib.CS_TYPE.get(dtype, 3)
+            if kind == 3:
                 raise _lib.CsError(f"states are read as float32, bfloat16 or float16, got {dtype}")
-            return torch.empty(shape, dtype=dtype, device=self.data.device)
-        if tuple(out.shape) != shape or out.dtype not in _lib.CS_TYPE or out.dtype == torch.float64 \
-                or (out.stride(3) != 1 and shape[3] > 1):
+            out = torch.empty(shape, dtype=dtype, device=self._data.device)
+            return out, kind, out.stride()
+        kind, strides = _lib.CS_TYPE.get(out.dtype, 3), out.stride()
+        if out.shape != shape or kind == 3 or (strides[-1] != 1 and shape[-1] > 1):
             raise _lib.CsError(f"out must be float32, bfloat16 or float16 {list(shape)} with adjacent values")
-        return out
+        return out, kind, strides
 
     def reorder(self, parents, steps=None):
         """The records of every chain follow ``parents`` [B,K] in place (``beam.reorder_states``), in the first ``steps`` slots
         (None: all)."""
         from .beam import reorder_states
-        data = self.data if steps is None else self.data[:int(steps)]
+        data = self._data if steps is None else self._data[:int(steps)]
         reorder_states(data, parents, batch_dim=1, out=data)
