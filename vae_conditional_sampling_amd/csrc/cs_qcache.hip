@@ -44,26 +44,54 @@ __device__ __forceinline__ void qc_store(QcBf16* p, float v) {   // nearest, tie
   p->u = (uint16_t)(v != v ? 0x7fc0u : (u + 0x7fffu + ((u >> 16) & 1)) >> 16);
 }
 
-// Codes of 8 values of a group whose largest finite magnitude is `top`; `fine`: all of the GROUP's values are finite.
-// The scale goes to `scale` (int8: a float's bits, else the byte).
-template <int FMT>
+// The largest of the lanes of a group (lg = 4, 8 or 16 neighbouring lanes): exchanges within quads, then the mirrored other
+// half of 8 and of 16 lanes, whose halves are of one value by then.
+__device__ __forceinline__ uint32_t qc_group_max(uint32_t v, int lg) {
+#define CS_STEP(CTRL_)                                                                                        \
+  {                                                                                                           \
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL_, 0xf, 0xf, false);         \
+    v = o > v ? o : v;                                                                                        \
+  }
+  CS_STEP(0xb1) CS_STEP(0x4e)            // quad_perm: 1 0 3 2, 2 3 0 1
+  if (lg > 4) CS_STEP(0x141)             // row_half_mirror
+  if (lg > 8) CS_STEP(0x140)             // row_mirror
+#undef CS_STEP
+  return v;
+}
+
+// Codes of 8 values of a group whose largest finite magnitude is `top`; `fine`: all of the GROUP's values are finite (PLAIN:
+// those of every group of the wavefront).  The scale goes to `scale` (int8: a float's bits, else the byte).
+template <int FMT, bool PLAIN>
 __device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, uint32_t* codes, uint32_t* scale) {
+  auto finite = [](float v) { return PLAIN || __builtin_fabsf(v) <= 3.402823466e+38f; };
   if (FMT == CS_QFMT_INT8) {
     const float s = fmaxf(top / 127.0f, 1.17549435e-38f);
     const float inv = 1.0f / s;
+    float q[QC_LANE];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < QC_LANE; ++i) {
+      const float v = (finite(x[i]) ? x[i] : 0.0f) * inv;
+      q[i] = __builtin_rintf(v);
+      near = near || __builtin_fabsf(v - q[i]) > 0.4999f;
+    }
+    if (__ballot(near)) {
+      // v is off by less than 2e-5, so these alone can be beside the nearest integer of the real quotient: the remainder
+      // x - q s is exact (a multiple of the last place of s or x, below 2^24 of them) and says so
+#pragma unroll
+      for (int i = 0; i < QC_LANE; ++i) {
+        const float v = finite(x[i]) ? x[i] : 0.0f;
+        const float r = 2.0f * __builtin_fmaf(-q[i], s, v);
+        const float away = __builtin_fabsf(r);
+        const bool odd = ((int)q[i] & 1) != 0;
+        if (away > s || (away == s && odd)) q[i] += r > 0.0f ? 1.0f : -1.0f;
+        q[i] = fminf(fmaxf(q[i], -127.0f), 127.0f);
+      }
+    }
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < QC_LANE; ++i) {
-      // x * inv is off by less than one, the remainder x - q s is exact (a multiple of the last place of s or x below
-      // 2^24 of them), so one correction gives the nearest integer of the real quotient
-      const float v = __builtin_fabsf(x[i]) <= 3.402823466e+38f ? x[i] : 0.0f;
-      float q = __builtin_rintf(v * inv);
-      const float r = 2.0f * __builtin_fmaf(-q, s, v);
-      const float away = __builtin_fabsf(r);
-      const bool odd = ((int)q & 1) != 0;
-      if (away > s || (away == s && odd)) q += r > 0.0f ? 1.0f : -1.0f;
-      q = fminf(fmaxf(q, -127.0f), 127.0f);
-      const uint32_t c = v == x[i] ? (uint32_t)(int)q & 0xffu : 0x80u;
+      const uint32_t c = finite(x[i]) ? (uint32_t)(int)q[i] & 0xffu : 0x80u;
       w[i >> 2] |= c << (8 * (i & 3));
     }
     codes[0] = w[0]; codes[1] = w[1];
@@ -78,10 +106,8 @@ __device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, 
   }
   float y[QC_LANE];
 #pragma unroll
-  for (int i = 0; i < QC_LANE; ++i) {
-    const bool ok = __builtin_fabsf(x[i]) <= 3.402823466e+38f;
-    y[i] = ok ? __builtin_amdgcn_ldexpf(x[i], -e) : (FMT == CS_QFMT_MXFP8 ? __builtin_nanf("") : 0.0f);
-  }
+  for (int i = 0; i < QC_LANE; ++i)
+    y[i] = finite(x[i]) ? __builtin_amdgcn_ldexpf(x[i], -e) : (FMT == CS_QFMT_MXFP8 ? __builtin_nanf("") : 0.0f);
   if (FMT == CS_QFMT_MXFP8) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -132,14 +158,12 @@ __device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale,
 
 // the slot of step i of a chain of a call that runs from `start` on; -1: not in the call
 __device__ __forceinline__ int32_t qc_slot(const QcArgs& a, uint32_t i, uint32_t chain) {
-  if (a.count && (int64_t)i >= a.count[chain]) return -1;
   const uint32_t T = a.by_T.d;
-  uint32_t s = (uint32_t)a.start0;               // (below T)
-  if (a.start) {
-    const int64_t far = a.start[chain];
-    if (far < 0) return -1;
-    s = far < (int64_t)T ? (uint32_t)far : (uint32_t)(far % (int64_t)T);
-  }
+  // (both asked for at once)
+  const int64_t count = a.count ? a.count[chain] : INT64_MAX;
+  const int64_t far = a.start ? a.start[chain] : a.start0;      // (start0 is below T)
+  if ((int64_t)i >= count || far < 0) return -1;
+  uint32_t s = far < (int64_t)T ? (uint32_t)far : (uint32_t)(far % (int64_t)T);
   s += i - cs_div(i, a.by_T) * T;
   return (int32_t)(s >= T ? s - T : s);
 }
@@ -164,82 +188,126 @@ template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
   const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
   const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
-  const bool live = ry < a.rows_per_block && row < a.rows;
-  const uint32_t i = live ? cs_div(row, a.by_chains) : 0, chain = live ? row - i * a.by_chains.d : 0;
-  const int32_t slot = live ? qc_slot(a, i, chain) : -1;
+  if (ry >= a.rows_per_block || row >= a.rows) return;
+  const uint32_t i = cs_div(row, a.by_chains), chain = row - i * a.by_chains.d;
+  const int32_t slot = qc_slot(a, i, chain);
+  if (slot < 0) return;                  // (all lanes of a row stay or leave, so the lanes of a group stay together)
   const uint32_t b = cs_div(chain, a.by_inner), k = chain - b * a.by_inner.d;
   const T* x = (const T*)a.x + i * a.stride[0] + b * a.stride[1] + k * a.stride[2];
-  char* rec = (char*)a.c.data + ((int64_t)(slot < 0 ? 0 : slot) * a.by_chains.d + chain) * a.record;
+  char* rec = (char*)a.c.data + ((int64_t)slot * a.by_chains.d + chain) * a.record;
   const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
-  // (lanes of a row: a multiple of the lanes of a group, which divide 64; whole groups of lanes take part or none)
+  // (lanes of a row: a multiple of the lanes of a group, which divide 64)
   for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
     const int d0 = l * QC_LANE;
     float v[QC_LANE];
-    float top = 0.0f;
-    bool fine = true;
-    if (slot >= 0 && d0 + QC_LANE <= D) {
+    if (d0 + QC_LANE <= D) {
       qc_load8(x + d0, v);
     } else {
 #pragma unroll
-      for (int e = 0; e < QC_LANE; ++e) v[e] = slot >= 0 && d0 + e < D ? qc_float(x[d0 + e]) : 0.0f;
+      for (int e = 0; e < QC_LANE; ++e) v[e] = d0 + e < D ? qc_float(x[d0 + e]) : 0.0f;
     }
+    // (magnitudes order as their bits do; infinities and NaN lie above all others)
+    constexpr uint32_t INFBITS = 0x7f800000u;
+    uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < QC_LANE; ++e) {
-      const float m = __builtin_fabsf(v[e]);
-      const bool ok = m <= 3.402823466e+38f;
-      top = fmaxf(top, ok ? m : 0.0f);
-      fine = fine && ok;
+      const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+      top = m > top ? m : top;
     }
-    int bad = fine ? 0 : 1;
-    for (int o = 1; o < lg; o <<= 1) {
-      top = fmaxf(top, __shfl_xor(top, o));
-      bad |= __shfl_xor(bad, o);
-    }
+    top = qc_group_max(top, lg);
     uint32_t codes[2] = {0, 0}, scale = 0;
-    qc_encode<FMT>(v, top, bad == 0, codes, &scale);
-    if (slot >= 0) {
-      const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
-      if (c0 < a.code_bytes) *(uint32_t*)(rec + c0) = codes[0];
-      if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) *(uint32_t*)(rec + c0 + 4) = codes[1];
-      if (l % lg == 0) {
-        if (FMT == CS_QFMT_INT8) *(uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) = scale;
-        else *(uint8_t*)(rec + a.code_bytes + l / lg) = (uint8_t)scale;
+    if (__ballot(top >= INFBITS) == 0) {
+      qc_encode<FMT, true>(v, __uint_as_float(top), true, codes, &scale);
+    } else {
+      const bool fine = top < INFBITS;
+      top = 0;
+#pragma unroll
+      for (int e = 0; e < QC_LANE; ++e) {
+        const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+        top = m > top && m < INFBITS ? m : top;
       }
+      top = qc_group_max(top, lg);
+      qc_encode<FMT, false>(v, __uint_as_float(top), fine, codes, &scale);
+    }
+    const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
+    if (c0 < a.code_bytes) *(uint32_t*)(rec + c0) = codes[0];
+    if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) *(uint32_t*)(rec + c0 + 4) = codes[1];
+    if (l % lg == 0) {
+      if (FMT == CS_QFMT_INT8) *(uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) = scale;
+      else *(uint8_t*)(rec + a.code_bytes + l / lg) = (uint8_t)scale;
     }
   }
 }
 
-template <int FMT, typename T>
+// R rows per lane, rows_per_block apart: their index loads, then their records, are under way together, where a call has
+// rows enough to fill the chip even so (a lane's chain of slot, record and store is some 5 us long).
+// PACKED: the rows of the call follow each other in `out` and their length is no multiple of 8 values.  Then the lanes' pieces
+// of a row would be stored in up to 8 parts each, every one of them touching all lines of the block's rows; the block's
+// rows are put together in LDS instead and stored as one run of 16-byte pieces.
+template <int FMT, typename T, int R, bool PACKED>
 __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  T* s_out = (T*)lds;                  // [R * rows_per_block][D]
   const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
-  const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
-  if (ry >= a.rows_per_block || row >= a.rows) return;
-  const uint32_t i = cs_div(row, a.by_chains), chain = row - i * a.by_chains.d;
-  const uint32_t b = cs_div(chain, a.by_inner), j = chain - b * a.by_inner.d;
-  const int64_t slot = a.slots ? a.slots[row] : qc_slot(a, i, chain);
-  const int64_t k = a.from ? a.from[row] : j;
-  const bool there = slot >= 0 && slot < a.c.T && k >= 0 && k < a.c.K;
-  const char* rec = (const char*)a.c.data + (there ? ((slot * a.c.B + b) * a.c.K + k) * a.record : 0);
-  T* out = (T*)a.out + i * a.stride[0] + b * a.stride[1] + j * a.stride[2];
+  const uint32_t row0 = blockIdx.x * (uint32_t)(R * a.rows_per_block);
+  const char* rec[R];
+  T* out[R];
+  bool live[R], there[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t row = row0 + r * a.rows_per_block + ry;
+    live[r] = ry < a.rows_per_block && row < a.rows;
+    const uint32_t at = live[r] ? row : 0, i = cs_div(at, a.by_chains), chain = at - i * a.by_chains.d;
+    const uint32_t b = cs_div(chain, a.by_inner), j = chain - b * a.by_inner.d;
+    const int64_t slot = a.slots ? a.slots[at] : qc_slot(a, i, chain);
+    const int64_t k = a.from ? a.from[at] : j;
+    there[r] = slot >= 0 && slot < a.c.T && k >= 0 && k < a.c.K;
+    rec[r] = (const char*)a.c.data + (there[r] ? ((slot * a.c.B + b) * a.c.K + k) * a.record : 0);
+    out[r] = PACKED ? s_out + (r * a.rows_per_block + ry) * a.c.D
+                    : (T*)a.out + i * a.stride[0] + b * a.stride[1] + j * a.stride[2];
+  }
   const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
   for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
     const int d0 = l * QC_LANE;
     if (d0 >= D) break;
-    uint32_t codes[2] = {0, 0}, scale = 127;
-    if (there) {
-      const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
-      codes[0] = *(const uint32_t*)(rec + c0);
-      if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) codes[1] = *(const uint32_t*)(rec + c0 + 4);
-      scale = FMT == CS_QFMT_INT8 ? *(const uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) : *(const uint8_t*)(rec + a.code_bytes + l / lg);
-    }
-    float v[QC_LANE];
-    qc_decode<FMT>(codes, scale, v);
-    if (d0 + QC_LANE <= D) {
-      qc_store8(out + d0, v);
-    } else {
+    uint32_t codes[R][2], scale[R];
 #pragma unroll
-      for (int e = 0; e < QC_LANE; ++e)
-        if (d0 + e < D) qc_store(out + d0 + e, v[e]);
+    for (int r = 0; r < R; ++r) {   // (the first record's bytes stand in for those of a row that does not exist)
+      const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
+      codes[r][0] = *(const uint32_t*)(rec[r] + c0);
+      codes[r][1] = FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes ? *(const uint32_t*)(rec[r] + c0 + 4) : 0;
+      scale[r] = FMT == CS_QFMT_INT8 ? *(const uint32_t*)(rec[r] + a.code_bytes + 4 * (l / lg)) : *(const uint8_t*)(rec[r] + a.code_bytes + l / lg);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v[QC_LANE];
+      qc_decode<FMT>(codes[r], scale[r], v);
+#pragma unroll
+      for (int e = 0; e < QC_LANE; ++e) v[e] = there[r] ? v[e] : 0.0f;
+      if (!live[r]) continue;
+      if (d0 + QC_LANE <= D) {
+        qc_store8(out[r] + d0, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < QC_LANE; ++e)
+          if (d0 + e < D) qc_store(out[r] + d0 + e, v[e]);
+      }
+    }
+  }
+  if (PACKED) {
+    __syncthreads();
+    const uint32_t rows = a.rows - row0 < (uint32_t)(R * a.rows_per_block) ? a.rows - row0 : (uint32_t)(R * a.rows_per_block);
+    const int n = (int)rows * D;
+    T* to = (T*)a.out + (int64_t)row0 * D;
+    constexpr int E = 16 / (int)sizeof(T);
+    for (int e = threadIdx.x * E; e < n; e += 256 * E) {
+      if (e + E <= n) {
+        uint32_t w[4];
+        __builtin_memcpy(w, __builtin_assume_aligned(s_out + e, 16), 16);
+        __builtin_memcpy(to + e, w, 16);
+      } else {
+        for (int f = e; f < n; ++f) to[f] = s_out[f];
+      }
     }
   }
 }
@@ -259,17 +327,22 @@ int check_qcache(const cs_qcache* c) {
   return CS_OK;
 }
 
-template <bool WRITE, int FMT>
-void launch_type(const QcArgs& a, int type, dim3 grid, hipStream_t st) {
-  if (WRITE) {
-    if (type == CS_TYPE_F32) hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, float>), grid, dim3(256), 0, st, a);
-    else if (type == CS_TYPE_BF16) hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, QcBf16>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, _Float16>), grid, dim3(256), 0, st, a);
+template <bool WRITE, int FMT, typename T>
+void launch_rows(const QcArgs& a, int R, bool packed, dim3 grid, hipStream_t st) {
+  const size_t lds = (size_t)a.rows_per_block * a.c.D * sizeof(T);   // (at most 256 * 8 values)
+  if constexpr (WRITE) {
+    hipLaunchKernelGGL((cs_qcache_write_kernel<FMT, T>), grid, dim3(256), 0, st, a);
   } else {
-    if (type == CS_TYPE_F32) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, float>), grid, dim3(256), 0, st, a);
-    else if (type == CS_TYPE_BF16) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, QcBf16>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, _Float16>), grid, dim3(256), 0, st, a);
+    if (packed) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, T, 1, true>), grid, dim3(256), lds, st, a);
+    else if (R == 4) hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, T, 4, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cs_qcache_read_kernel<FMT, T, 1, false>), grid, dim3(256), 0, st, a);
   }
+}
+template <bool WRITE, int FMT>
+void launch_type(const QcArgs& a, int type, int R, bool packed, dim3 grid, hipStream_t st) {
+  if (type == CS_TYPE_F32) launch_rows<WRITE, FMT, float>(a, R, packed, grid, st);
+  else if (type == CS_TYPE_BF16) launch_rows<WRITE, FMT, QcBf16>(a, R, packed, grid, st);
+  else launch_rows<WRITE, FMT, _Float16>(a, R, packed, grid, st);
 }
 
 // n steps of B * inner rows
@@ -289,10 +362,14 @@ int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStr
   a.lanes = (c.D + c.group - 1) / c.group * (c.group / QC_LANE);
   a.by_lanes = cs_div_by(a.lanes);
   a.rows_per_block = a.lanes >= 256 ? 1 : 256 / a.lanes;
-  const dim3 grid((a.rows + a.rows_per_block - 1) / a.rows_per_block);
-  if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, grid, st);
-  else if (c.fmt == CS_QFMT_MXFP8) launch_type<WRITE, CS_QFMT_MXFP8>(a, type, grid, st);
-  else launch_type<WRITE, CS_QFMT_MXFP4>(a, type, grid, st);
+  const uint32_t blocks = (a.rows + a.rows_per_block - 1) / a.rows_per_block;
+  const bool packed = !WRITE && c.D % QC_LANE != 0 && a.lanes <= 16 && a.stride[2] == c.D && a.stride[1] == (int64_t)inner * c.D &&
+                      (n == 1 || a.stride[0] == c.B * inner * c.D);
+  const int R = WRITE || packed || blocks < 8192 ? 1 : 4;
+  const dim3 grid((blocks + R - 1) / R);
+  if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, R, packed, grid, st);
+  else if (c.fmt == CS_QFMT_MXFP8) launch_type<WRITE, CS_QFMT_MXFP8>(a, type, R, packed, grid, st);
+  else launch_type<WRITE, CS_QFMT_MXFP4>(a, type, R, packed, grid, st);
   CS_HIP(hipGetLastError());
   return CS_OK;
 }
