@@ -336,20 +336,25 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
 __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, int cap) {
   extern __shared__ char lds[];
   double* s_beam = (double*)lds;                                    // [K] what a kept logit of the beam gets added
-  uint64_t* s_key = (uint64_t*)(lds + ((a.c.K * 8 + 15) & ~15));    // [cap]
-  int64_t* s_at = (int64_t*)(s_key + cap);                          // [cap] k*V + v
+  uint64_t* s_key = (uint64_t*)(lds + ((a.c.K * 8 + 15) & ~15));    // [cap] scores of candidates, as ordered bits
+  int64_t* s_at = (int64_t*)(s_key + cap);                          // [cap] k << 32 | v
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
-  __shared__ int s_n;
+  int* s_open = (int*)(s_at + cap);                                 // [threads] stretches to go through
+  __shared__ int s_n, s_left;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, waves = threads >> 6;
   const int64_t b = blockIdx.x;
   const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
-  const int64_t V = a.c.V;
   const int32_t total = K * C;         // (at most 2^31 / keep, checked on the host)
   const BmStat* stat = a.stat + b * total;
   const BmItem* item = a.item + b * total * keep;
-  if (tid == 0) s_n = 0;
+  constexpr double INF = __builtin_inf();
+  // (asked for before the normalisers are formed)
+  const float top0 = tid < total ? stat[tid].top : -__builtin_inff();
+  const int n0 = tid < total ? stat[tid].n : 0;
+  const int n_first = total <= 64 && lane < total ? stat[lane].n : 0;
+  if (tid == 0) { s_n = 0; s_left = 0; }
   for (int k = wave; k < K; k += waves) {
     const int64_t row = b * K + k;
     double before = 0.0;
@@ -357,96 +362,106 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     if (a.c.normalise && !(a.finished && a.finished[row])) {
       const BmStat* st = stat + k * C;
       // lanes join their stretches, then each other
-      double ref = -__builtin_inf(), sum = 0.0;
+      double ref = -INF, sum = 0.0;
       for (int c = lane; c < C; c += 64) {
         const BmStat s = st[c];
         if (s.sum != s.sum) sum = s.sum;             // (NaN stays)
         if (!(s.top > -__builtin_inff())) continue;  // nothing allowed there
         const double m = fmax(ref, s.ref);
-        sum = sum * exp(ref - m) + s.sum * exp(s.ref - m);
+        sum = sum * (ref == m ? 1.0 : exp(ref - m)) + s.sum * (s.ref == m ? 1.0 : exp(s.ref - m));
         ref = m;
       }
       double m = ref;
-      for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
-      sum = bm_wave_sum(ref > -__builtin_inf() ? sum * exp(ref - m) : sum);
+      if (__ballot(ref != 0.0))        // (the rule: all within +-690, so of reference 0)
+        for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+      sum = bm_wave_sum(ref > -INF && ref != m ? sum * exp(ref - m) : sum);
       before -= m + log(sum);          // (+inf, NaN or nothing allowed: NaN or +inf, with no candidate left to count)
     }
     if (lane == 0) s_beam[k] = before;
   }
   __syncthreads();
   auto key_of = [&](float x, int g) { return bm_key64((double)x + s_beam[cs_div(g, a.by_stretches)]); };
-  // a bound from below in two steps.  First the W-th largest score, as far as its leading 32 bits say, among the lanes' best
-  // of a wavefront: of the stretches' largest logits or, where these are few, of all kept ones.
-  const bool by_stretch = total >= 4 * W;
-  uint32_t best = 0;
-  if (by_stretch) {
-    for (int g = tid; g < total; g += threads) {
-      const float x = stat[g].top;
-      const uint32_t key = x > -__builtin_inff() ? (uint32_t)(key_of(x, g) >> 32) : 0u;
-      best = key > best ? key : best;
-    }
-  } else {
-    for (int i = tid; i < total * keep; i += threads) {
-      const int g = cs_div(i, a.by_keep);
-      if (i - g * keep < stat[g].n) {
-        const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
+  // a bound from below; none where there are few candidates
+  uint64_t t = 1;
+  if (total > 64 || bm_wave_sum((double)n_first) > cap / 2) {
+    // the W-th largest score, as far as its leading 32 bits say, among the lanes' best of a wavefront: of the stretches' largest
+    // logits or, where these are few, of all kept ones
+    uint32_t best = 0;
+    if (total >= 4 * W) {
+      for (int g = tid; g < total; g += threads) {
+        const float x = g == tid ? top0 : stat[g].top;
+        const uint32_t key = x > -__builtin_inff() ? (uint32_t)(key_of(x, g) >> 32) : 0u;
         best = key > best ? key : best;
       }
+    } else {
+      for (int i = tid; i < total * keep; i += threads) {
+        const int g = cs_div(i, a.by_keep);
+        if (i - g * keep < stat[g].n) {
+          const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
+          best = key > best ? key : best;
+        }
+      }
     }
+    const uint32_t t_wave = bm_wave_threshold<32>(best, W);
+    if (lane == 0) s_wave[wave] = t_wave;
+    __syncthreads();
+    uint32_t t32 = 1;
+    for (int w = 0; w < waves; ++w) t32 = s_wave[w] > t32 ? (uint32_t)s_wave[w] : t32;
+    // where many of the lanes' best are left, the W-th largest of these (4 us; ranking the hundreds of candidates that are above the first bound took 10)
+    const uint64_t reach = __ballot(best >= t32);
+    if (waves > 1) {
+      if (lane == 0) atomicAdd(&s_left, __popcll(reach));
+      __syncthreads();
+      const int left = s_left;
+      if (left > 4 * W) {
+        uint32_t* s_best = (uint32_t*)s_key;           // [threads] (threads <= 2 cap)
+        if (best >= t32) s_best[atomicAdd(&s_n, 1)] = best;
+        __syncthreads();
+        if (tid == 0) { s_n = 0; s_wave[0] = t32; }
+        __syncthreads();
+        if (tid < left) {
+          const uint32_t mine = s_best[tid];
+          int before = 0;
+          for (int j = 0; j < left; ++j) before += s_best[j] > mine || (s_best[j] == mine && j < tid);
+          if (before == W - 1) s_wave[0] = mine;
+        }
+        __syncthreads();
+        t32 = (uint32_t)s_wave[0];
+      }
+    }
+    t = t32 > 1 ? (uint64_t)t32 << 32 : 1;
   }
-  const uint32_t t_wave = bm_wave_threshold<32>(best, W);
-  if (lane == 0) s_wave[wave] = t_wave;
-  __syncthreads();
-  uint32_t t32 = 1;
-  for (int w = 0; w < waves; ++w) t32 = s_wave[w] > t32 ? (uint32_t)s_wave[w] : t32;
-  // Then, with several wavefronts, the W-th largest of the lanes' best that are left.
-  if (waves > 1) {
-    uint32_t* s_best = (uint32_t*)s_key;           // [threads] (threads <= 2 cap)
-    if (tid == 0) s_n = 0;
+  // stretches whose largest logit reaches the bound are gone through by 16 lanes each
+  for (int g0 = 0; g0 < total; g0 += threads) {
     __syncthreads();
-    if (best >= t32) s_best[atomicAdd(&s_n, 1)] = best;
+    if (tid == 0) s_left = 0;
     __syncthreads();
-    const int left = s_n;
-    __syncthreads();
-    if (tid == 0) { s_n = 0; s_wave[0] = t32; }
-    __syncthreads();
-    if (left > W && tid < left) {
-      const uint32_t mine = s_best[tid];
-      int before = 0;
-      for (int j = 0; j < left; ++j) before += s_best[j] > mine || (s_best[j] == mine && j < tid);
-      if (before == W - 1) s_wave[0] = mine;
+    const int g = g0 + tid;
+    if (g < total) {
+      const float x = g0 == 0 ? top0 : stat[g].top;
+      if (x > -__builtin_inff() && key_of(x, g) >= t) s_open[atomicAdd(&s_left, 1)] = g;
     }
     __syncthreads();
-    t32 = (uint32_t)s_wave[0];
-  }
-  const uint64_t t = t32 > 1 ? (uint64_t)t32 << 32 : 1;
-  auto offer = [&](const BmItem& i, int g) {
-    const uint64_t key = key_of(i.x, g);
-    if (key < t) return;
-    const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
-    if (at < cap) { s_key[at] = key; s_at[at] = (int64_t)cs_div(g, a.by_stretches) * V + i.v; }
-  };
-  // a wavefront looks at 64 stretches and then, together, through each whose largest logit reaches the bound
-  for (int g0 = wave * 64; g0 < total; g0 += threads) {
-    const int g = g0 + lane;
-    const float x = g < total ? stat[g].top : -__builtin_inff();
-    const int n_mine = g < total ? stat[g].n : 0;
-    uint64_t q = __ballot(n_mine > 0 && x > -__builtin_inff() && key_of(x, g) >= t);
-    while (q) {
-      const int s = (int)__ffsll((unsigned long long)q) - 1;
-      q &= q - 1;
-      const int n = __shfl(n_mine, s);
-      for (int r = lane; r < n; r += 64) offer(item[(int64_t)(g0 + s) * keep + r], g0 + s);
+    const int open = s_left;
+    for (int o = tid >> 4; o < open; o += threads >> 4) {
+      const int h = s_open[o], n = g0 == 0 && h == tid ? n0 : stat[h].n;
+      for (int r = tid & 15; r < n; r += 16) {
+        const BmItem i = item[(int64_t)h * keep + r];
+        const uint64_t key = key_of(i.x, h);
+        if (key < t) continue;
+        const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
+        if (at < cap) { s_key[at] = key; s_at[at] = (int64_t)cs_div(h, a.by_stretches) << 32 | i.v; }
+      }
     }
   }
   __syncthreads();
   auto put = [&](int w, uint64_t key, int64_t at) {
     const int64_t o = b * W + w;
-    const double s = key ? bm_value64(key) : -__builtin_inf();
+    const double s = key ? bm_value64(key) : -INF;
     if (a.c.scores_type == CS_TYPE_F64) ((double*)a.out_scores)[o] = s;
     else ((float*)a.out_scores)[o] = (float)s;
-    a.parents[o] = key ? at / V : (w < K ? w : K - 1);
-    a.tokens[o] = key ? at % V : -1;
+    a.parents[o] = key ? at >> 32 : (w < K ? w : K - 1);
+    a.tokens[o] = key ? at & 0xffffffff : -1;
   };
   const int n = s_n;
   if (n <= cap) {
@@ -470,7 +485,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
       const int g = cs_div(i, a.by_keep);
       if (i - g * keep >= stat[g].n) continue;
       const uint64_t u = key_of(item[i].x, g);
-      const int64_t f = (int64_t)cs_div(g, a.by_stretches) * V + item[i].v;
+      const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item[i].v;
       if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
     }
     for (int o = 32; o; o >>= 1) {
@@ -565,14 +580,16 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, grid, st);
   else launch_scan<_Float16>(a, grid, st);
   CS_HIP(hipGetLastError());
-  // places for what reaches the joined bound
-  const int cap = c->W * 32 < 512 ? 512 : c->W * 32 > 2048 ? 2048 : c->W * 32;
   // a wavefront per beam and a thread per stretch, as far as that goes
   int64_t waves = ((int64_t)c->K * a.stretches + 63) / 64;
   waves = waves > c->K ? waves : c->K;
   const int threads = 64 * (int)(waves < BM_JOIN / 64 ? waves : BM_JOIN / 64);
-  hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads), (size_t)(((c->K * 8 + 15) & ~15) + cap * 16), st, a,
-                     cap);
+  // places for what reaches the joined bound
+  const int least = threads == 64 ? 128 : 1024;
+  int cap = c->W * 32;
+  cap = cap < least ? least : cap > 2048 ? 2048 : cap;
+  hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads),
+                     (size_t)(((c->K * 8 + 15) & ~15) + cap * 16 + threads * 4), st, a, cap);
   CS_HIP(hipGetLastError());
   return CS_OK;
 }
