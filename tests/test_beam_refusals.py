@@ -127,3 +127,16 @@ def test_wrappers_refuse_cpu_tensors_shapes_and_types():
         q.read(p.int())
     with pytest.raises(_lib.CsError, match="out must be"):
         q.read(p, out=torch.zeros(2, 3, 8))
+
+
+def test_sampler_options_are_checked():
+    from vae_conditional_sampling_amd.sampling.test_step_vae_sampling import TestVAELatentAdaptiveImportanceResampling as S
+    kw = dict(num_iterations=3, num_imp_samples=1, weighting_scheme="dmis", resampling_scheme="gr", resampling_method="multinomial",
+              num_copies=4, store_last_n_iterations=-1, store_every_n_iterations=1, imputation_metric_quantiles=[],
+              compute_f1_metric=False, compute_inv_f1_metric=False, compute_bin_accuracy_metric=False, compute_rmse_metric=False,
+              compute_ssim_metric=False, compute_latent_wass_metric=False, imputation_fn="vae_samples")
+    for bad in (dict(resample_final_imps_method="beam"), dict(resample_final_imps_method="top"),
+                dict(resample_final_imps_method="top", resample_final_imps_num_samples=65),
+                dict(imputation_history_format="int4")):
+        with pytest.raises(NotImplementedError):
+            S(**kw, **bad).on_test_start()

@@ -30,6 +30,7 @@ from .. import _lib
 from ..utils.artifacts import AsyncNpzWriter
 from ..utils.hparams import HyperparametersMixin
 from . import engine, imputation_metrics
+from .beam import MAX_WIDTH, beam_select
 from .utils import ImputationHistoryQueue, ImputationHistoryQueue_with_restrictedavailability
 from .vae_imputation import (importance_resampling_gibbs_iteration, pseudo_gibbs_iteration,
                              standard_importance_resampling)
@@ -436,24 +437,40 @@ def _means_of_three(a, b, c):
     return a.mean(), b.mean(), c.mean()
 
 
-def _final_resampling(self, proposals, X_true, M, num_samples):
+def _final_draws(src, lw, Zp, n, rng):
+    """(idx[B,n], Z[B,n,Zd]) of n draws per example from the Categorical over its proposals."""
+    import ctypes as C
+    T, I, B, Kp, Zd = Zp.shape
+    dev = Zp.device
+    u = src.uniform64(B, n).to(dev).contiguous() if src is not None else None
+    cdf = torch.empty(B, T * I * Kp, device=dev)
+    idx = torch.empty(B, n, device=dev, dtype=torch.int64)
+    Zout = torch.empty(B, n, Zd, device=dev)
+    _lib.check(_lib.lib().cs_final_resample(_lib.ptr(lw), _lib.ptr(Zp), T * I, B, Kp, Zd, _lib.ptr(u),
+                                            C.byref(rng), n, _lib.ptr(cdf), _lib.ptr(idx), _lib.ptr(Zout),
+                                            _lib.current_stream()))
+    return idx, Zout
+
+
+def _final_resampling(self, proposals, X_true, M, num_samples, method='multinomial'):
     """Categorical over all stored proposals of every example, ``n`` draws, decode in one launch,
     sample and set the observed values (test_step_vae_sampling.py:1991-2032, 2151-2185).
-    ``proposals`` = (Z[T,I,B,K',Zd], log_w[T,I,B,K']) on the device."""
-    import ctypes as C
+    ``proposals`` = (Z[T,I,B,K',Zd], log_w[T,I,B,K']) on the device.  ``method`` 'top' (no counterpart in the reference):
+    the n proposals of the largest weights instead of draws, best first, equal ones in the order of '(t i k)'; where fewer
+    have a weight the best is repeated."""
     Zp, lw = proposals
     T, I, B, Kp, Zd = Zp.shape
     n = T * Kp if num_samples is None else num_samples
     dev = Zp.device
     src = self.draw_source
-    u = src.uniform64(B, n).to(dev).contiguous() if src is not None else None
-    cdf = torch.empty(B, T * I * Kp, device=dev)
-    idx = torch.empty(B, n, device=dev, dtype=torch.int64)
-    Zout = torch.empty(B, n, Zd, device=dev)
     rng = _lib.make_rng(self.rng_seed, 0, self.example_offset)
-    _lib.check(_lib.lib().cs_final_resample(_lib.ptr(lw), _lib.ptr(Zp), T * I, B, Kp, Zd, _lib.ptr(u),
-                                            C.byref(rng), n, _lib.ptr(cdf), _lib.ptr(idx), _lib.ptr(Zout),
-                                            _lib.current_stream()))
+    if method == 'top':
+        weights = lw.reshape(T * I, B, Kp).permute(1, 0, 2).reshape(B, 1, T * I * Kp)
+        idx = beam_select(None, weights, n, normalise=False).tokens   # (weights of one example: no normaliser is needed)
+        idx = torch.where(idx < 0, idx[:, :1], idx).clamp(min=0)
+        Zout = Zp.reshape(T * I, B, Kp, Zd)[idx // Kp, torch.arange(B, device=dev)[:, None], idx % Kp]
+    else:
+        idx, Zout = _final_draws(src, lw, Zp, n, rng)
     gen = engine.decode_params(self.model, Zout.reshape(B * n, Zd))
     D = X_true.shape[-1]
     Xz = X_true.to(dev, torch.float32).unsqueeze(1).repeat(1, n, 1).contiguous()
@@ -492,6 +509,7 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
                  num_historical_proposals: int = None,
                  no_historic_proposals_iterations: int = None,
                  imputation_history_length: int = None,
+                 imputation_history_format: str = None,   # int8 | mxfp8 | mxfp4: the history in 8 or 4 bits
 
                  use_miss_model: bool = False,
                  accept_reject_xm: bool = False,
@@ -500,6 +518,7 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
 
                  resample_final_imps: bool = False,
                  resample_final_imps_num_samples: int = None,
+                 resample_final_imps_method: str = 'multinomial',   # top: the proposals of the largest weights, best first
                  **kwargs
                  ):
         super().__init__(*args, **kwargs)
@@ -512,6 +531,13 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
     def on_test_start(self):
         super().on_test_start()
         hp = self.hparams
+        if hp.resample_final_imps_method not in ('multinomial', 'top'):
+            raise NotImplementedError(f'Method not implemented for {hp.resample_final_imps_method = }')
+        if hp.resample_final_imps_method == 'top' and not 1 <= (hp.resample_final_imps_num_samples or 0) <= MAX_WIDTH:
+            raise NotImplementedError(f"resample_final_imps_method 'top' keeps 1 to {MAX_WIDTH} proposals: set "
+                                      "resample_final_imps_num_samples")
+        if hp.imputation_history_format not in (None, *_lib.CS_QFMT):
+            raise NotImplementedError(f'Method not implemented for {hp.imputation_history_format = }')
         if hp.use_miss_model or hp.accept_reject_xm:
             raise NotImplementedError("missingness models (MNAR) are not implemented")
         _lib.proposal_transform_args(hp.var_proposal_temperature, hp.var_proposal_anneal_type_to_prior)
@@ -574,7 +600,8 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
         history = None
         if hp.num_historical_proposals is not None:   # :1866-1870
             history = ImputationHistoryQueue(max_history_length=hp.imputation_history_length, batch_shape=X.shape,
-                                             dtype=torch.bool if _check_if_bool(X) else torch.float32, device=X.device)
+                                             dtype=torch.bool if _check_if_bool(X) else torch.float32, device=X.device,
+                                             storage=hp.imputation_history_format)
         clip_min = clip_max = None
         if hp.clip_imputations:
             X_temp = X[:, 0].clone()
@@ -693,7 +720,8 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
     def final_resampling(self, X_true, M):
         """Resample the latents across all iterations and decode (:1991-2032).  Returns
         ``(imputations[1,B,n,D], latents[B,n,Zd], idx[B,n])`` as device tensors."""
-        return _final_resampling(self, self._proposals, X_true, M, self.hparams.resample_final_imps_num_samples)
+        return _final_resampling(self, self._proposals, X_true, M, self.hparams.resample_final_imps_num_samples,
+                                 self.hparams.resample_final_imps_method)
 
     def on_test_batch_end(self, outputs, batch: Any, batch_idx: int, dataloader_idx: int = 0) -> None:
         super().on_test_batch_end(outputs, batch, batch_idx, dataloader_idx)

@@ -19,11 +19,15 @@ class ImputationHistoryQueue(object):
     """Ring ``[T,B,K,D]`` of past imputations in HBM with the reference's stratified sampling
     (irwg/sampling/utils.py:5-68).  The host tracks ``tail_idx`` / ``full`` and computes the H ring
     slots of a draw (they are common to the batch); the gather of the chosen imputations into the
-    proposal set runs on the device (``cs_history_concat``)."""
+    proposal set runs on the device (``cs_history_concat``).
 
-    def __init__(self, max_history_length, batch_shape, dtype=torch.float32, device="cuda"):
-        if dtype not in (torch.float32, torch.bool):
-            raise NotImplementedError(f"history dtype {dtype}")
+    ``storage`` (``int8`` | ``mxfp8`` | ``mxfp4``; no counterpart in the reference): the ring holds the imputations in 8 or 4
+    bits (``QuantisedHistory``), for real-valued data whose float32 ring would not fit; slots and chains are drawn as for
+    the float32 ring, the historical proposals are what the ring reads back."""
+
+    def __init__(self, max_history_length, batch_shape, dtype=torch.float32, device="cuda", storage=None):
+        if dtype not in (torch.float32, torch.bool) or (storage is not None and dtype == torch.bool):
+            raise NotImplementedError(f"history dtype {dtype}" + (f" with storage {storage}" if storage else ""))
         self.max_history_length = int(max_history_length)
         self.tail_idx = -1
         self.full = False
@@ -31,6 +35,12 @@ class ImputationHistoryQueue(object):
         B, K, D = self.batch_shape
         # dtype bool (the reference's queue for binary data, which stores X.bool()): a uint8 ring holding x != 0
         self.u8 = dtype == torch.bool
+        self.quantised = None
+        if storage is not None:
+            self.quantised = QuantisedHistory(self.max_history_length, self.batch_shape, storage, device=device)
+            self.history_queue = self.quantised.data
+            self._chain_ids = None
+            return
         self.history_queue = torch.empty((self.max_history_length, B, K, D),
                                          dtype=torch.uint8 if self.u8 else torch.float32, device=device)
 
@@ -47,6 +57,9 @@ class ImputationHistoryQueue(object):
         B, K, D = self.batch_shape
         X = X.to(self.history_queue.device, torch.float32).contiguous()
         self._increment_tail()
+        if self.quantised is not None:
+            self.quantised.write(X, self.tail_idx)
+            return
         fn = _lib.lib().cs_history_enqueue_u8 if self.u8 else _lib.lib().cs_history_enqueue
         _lib.check(fn(_lib.ptr(self.history_queue), None, self.max_history_length, self.tail_idx, 0, _lib.ptr(X), B, K, D,
                       _lib.current_stream()))
@@ -68,6 +81,17 @@ class ImputationHistoryQueue(object):
         B, K, D = self.batch_shape
         H = len(slots)
         Xc = out if out is not None else torch.empty(B, K + H, D, device=X.device, dtype=torch.float32)
+        if self.quantised is not None:
+            Xc[:, :K] = X
+            at = torch.tensor(slots, device=X.device).expand(B, H)
+            if chain_of_proposal is not None:
+                chains = torch.tensor([int(c) for c in chain_of_proposal], device=X.device).expand(B, H)
+            elif chain_of_example is not None:
+                chains = chain_of_example.to(X.device, torch.int64)[:, None].expand(B, H)
+            else:
+                chains = self._drawn_chains(H, rng)
+            self.quantised.read(at, chains, out=Xc[:, K:])
+            return Xc
         i32 = C.c_int32 * H
         cop = i32(*[int(c) for c in chain_of_proposal]) if chain_of_proposal is not None else None
         coe = chain_of_example.to(X.device, torch.int64).contiguous() if chain_of_example is not None else None
@@ -76,6 +100,19 @@ class ImputationHistoryQueue(object):
         _lib.check(fn(_lib.ptr(X), _lib.ptr(self.history_queue), B, K, D, H, i32(*slots), cop, _lib.ptr(coe), C.byref(rng),
                       _lib.ptr(Xc), _lib.current_stream()))
         return Xc
+
+
+    def _drawn_chains(self, H, rng):
+        """[B,H]: the chain per example that the counter RNG gives ``cs_history_concat``, by that call on a ring of chain
+        numbers."""
+        B, K, _ = self.batch_shape
+        if self._chain_ids is None:
+            self._chain_ids = torch.arange(K, device=self.history_queue.device, dtype=torch.float32).expand(1, B, K).contiguous()
+        ids, got = self._chain_ids, torch.empty(B, K + 1, device=self.history_queue.device)
+        rng = rng if rng is not None else _lib.make_rng(0)
+        _lib.check(_lib.lib().cs_history_concat(_lib.ptr(ids), _lib.ptr(ids), B, K, 1, 1, (C.c_int32 * 1)(0), None, None, C.byref(rng),
+                                                _lib.ptr(got), _lib.current_stream()))
+        return got[:, K:].long().expand(B, H)
 
 
 def glr_history_chain_idx(K, num_historical_proposals, glr_cluster_size):
