@@ -249,3 +249,43 @@ def test_states_of_more_than_4_gib():
     want = tag[:, torch.arange(B, device="cuda")[:, None], p]
     assert torch.equal(x[..., :1], want) and torch.equal(x[..., -1:], want) and torch.equal(x[..., 12345:12346], want)
     assert bool((x[-1] == want[-1]).all())
+
+
+def test_logits_and_masks_beyond_4_gib():
+    far = (1 << 32) + 12345                                                              # elements between the examples
+    big = torch.empty(2 * far, dtype=torch.bfloat16, device="cuda")
+    big[:1], big[far:far + 1] = 0, 0
+    logits = big.as_strided((2, 3, 3000), (far, 3000, 1))
+    g = torch.Generator().manual_seed(6)
+    logits.copy_((torch.randn(2, 3, 3000, generator=g) * 2).cuda())
+    held = big.view(torch.uint8).as_strided((2, 3, 3000), (2 * far - 4096, 3000, 1), 100000)
+    mask = torch.rand(2, 3, 3000, generator=g) < 0.5
+    held.copy_(mask)
+    check(beam_select(None, logits, 9, mask=held), None, logits.cpu(), 9, mask=mask)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_logits_of_every_magnitude(dtype):
+    """The normaliser where the sums of single stretches would leave the range of their type: all logits far below or above
+    zero, and stretches of one beam that lie far apart."""
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(9, 2, 5000, generator=g) * 2
+    for b, shift in enumerate((-689.0, -601.0, -599.0, 599.0, 601.0, 5000.0, -5000.0)):
+        x[b] += shift
+    x[7, :, :2048] += 900
+    x[7, :, 4096:] -= 900
+    x[8] *= 300
+    logits = x.to(dtype).cuda()
+    scores = torch.zeros(9, 2, dtype=torch.float64, device="cuda")
+    check(beam_select(scores, logits, 7), scores, logits, 7)
+    mask = (torch.rand(9, 1, 5000, generator=g) < 0.3).cuda()
+    check(beam_select(scores, logits, 7, mask=mask), scores, logits, 7, mask=mask)
+
+
+@pytest.mark.parametrize("W", [33, 48, 64])
+@pytest.mark.parametrize("B,K,V", [(1, 1, 2048), (2, 40, 64), (1, 3, 6000), (1, 64, 3000), (3, 2, 33000)])
+def test_wide_searches(B, K, V, W):
+    scores, logits, _ = make(B, K, V, torch.bfloat16, V + W)                             # (many equal values)
+    check(beam_select(scores, logits, W), scores, logits, W)
+    rows = logits.round()                                                                # (a dozen distinct ones)
+    check(beam_select(scores, rows, W), scores, rows, W)

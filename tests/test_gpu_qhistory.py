@@ -96,6 +96,20 @@ def test_integers_of_random_scales_round_to_the_nearest(fmt, group):
 
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
+def test_the_largest_of_a_group_chooses_its_scale(fmt, group):
+    """Largest magnitudes on, below and above the end of the elements' range and of powers of two."""
+    ends = np.float32([448.0, 6.0, 127.0, 1.0, 256.0, 0.75, 0.875, 3.0])
+    tops = np.concatenate([ends, np.nextafter(ends, np.float32(0)), np.nextafter(ends, np.float32(1e9))])
+    tops = np.concatenate([(tops * np.float32(s)).astype(np.float32) for s in (1.0, 2.0 ** -60, 2.0 ** 70, 2.0 ** -120)])
+    x = np.random.RandomState(1).uniform(-1, 1, (len(tops), group)).astype(np.float32) * tops[:, None]
+    x[:, 5] = -tops
+    t = torch.from_numpy(x).reshape(len(tops), 1, 1, group)
+    q = QuantisedHistory(len(tops), (1, 1, group), fmt, group=group)
+    q.write(t.cuda(), 0)
+    close(q.read_steps(0, len(tops))[:, 0, 0], O.quantised(x, fmt, group), fmt)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
 def test_zeros_tiny_huge_and_not_finite_values(fmt, group):
     inf, nan, f = float("inf"), float("nan"), torch.finfo(torch.float32)
     D = 2 * group + 5

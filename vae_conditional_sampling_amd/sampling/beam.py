@@ -94,6 +94,8 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
         finished = finished.contiguous()
         finished_at = finished.data_ptr()
     width = int(width)
+    if not 1 <= width <= MAX_WIDTH:
+        raise _lib.CsError(f"width must be 1 .. {MAX_WIDTH}, got {width}")
     cfg, nbytes = _select_cfg(B, K, V, width, logits_type, _lib.CS_TYPE[out_type], int(bool(normalise)), int(end_token), ls[0],
                               ls[1], ms[0], ms[1])
     # the workspace is the call's own (calls on several streams and captured ones share nothing)
