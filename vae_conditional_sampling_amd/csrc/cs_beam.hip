@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
         if (tid < left) {
           const uint32_t mine = s_best[tid];
           int before = 0;
+#pragma unroll 8
           for (int j = 0; j < left; ++j) before += s_best[j] > mine || (s_best[j] == mine && j < tid);
           if (before == W - 1) s_wave[0] = mine;
         }
@@ -477,6 +478,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
       const uint64_t key = s_key[i];
       const int64_t at = s_at[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += s_key[j] > key || (s_key[j] == key && s_at[j] < at);
       if (rank < W) put(rank, key, at);
     }
