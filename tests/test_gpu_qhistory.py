@@ -205,6 +205,8 @@ def test_strides_and_windows():
         assert torch.equal(wide[:, :, 1:K + 1, 2:D + 2], ref.to(dtype))
         wide[:, :, 1:K + 1, 2:D + 2] = 7.0
         assert bool((wide == 7.0).all())             # nothing around the window
+    with pytest.raises(_lib.CsError, match="place of its own"):
+        q.read(slots, out=torch.zeros(1, B, K, D, device="cuda").expand(5, B, K, D))
     assert torch.equal(q.read_steps(4, 9), q.read(((4 + torch.arange(9)) % T)[:, None, None].expand(9, B, K).cuda()))
     assert q.read(slots[:0]).shape == (0, B, K, D)
     empty = QuantisedHistory(3, (0, 2, 5), "mxfp4")

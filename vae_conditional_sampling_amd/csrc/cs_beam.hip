@@ -294,24 +294,31 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
       if (n <= keep && x[i] >= t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
     }
   }
-  if (n > keep) {   // many equal or ascending values: the W-th largest of all, bit by bit
-    uint32_t u = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const float f = bm_value(u | (1u << bit));   // (patterns of NaN reach nothing)
-      int c = 0;
+  if (n > keep) {
+    // too many (W above 32, ascending or equal values): bisect for a bound that W to `keep` of them reach
+    uint32_t lo = bm_key(t), hi = bm_key(top) + 1;   // W or more reach lo, none hi
+    int c = n;
+    while (c > keep && hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const float f = bm_value(mid);
+      int reach = 0;
 #pragma unroll
-      for (int i = 0; i < LANE; ++i) c += __popcll(__ballot(x[i] >= f));
-      if (c >= W) u |= 1u << bit;
+      for (int i = 0; i < LANE; ++i) reach += __popcll(__ballot(x[i] >= f));
+      if (reach < W) hi = mid;
+      else { lo = mid; c = reach; }
     }
-    t = bm_value(u);
+    t = bm_value(lo);
+    const bool equal = c > keep;       // none found: lo is the W-th largest value, and others equal it
     n = 0;
 #pragma unroll
     for (int i = 0; i < LANE; ++i) {
-      const uint64_t m = __ballot(x[i] > t);
-      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-      if (x[i] > t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
+      const bool take = equal ? x[i] > t : x[i] >= t;
+      const uint64_t m = __ballot(take);
+      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
+      if (take) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
       n += __popcll(m);
     }
+    if (equal) {
     // of those equal to it the first ones
 #pragma unroll
     for (int j = 0; j < LANE / N; ++j) {
@@ -333,6 +340,7 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
       n += __shfl(incl, 63);
     }
     n = n < W ? n : W;
+    }
   }
   if (lane == 0) a.stat[item] = BmStat{ref, sum, top, n};
 }
@@ -346,7 +354,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   int64_t* s_at = (int64_t*)(s_key + cap);                          // [cap] k << 32 | v
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
-  int* s_open = (int*)(s_at + cap);                                 // [threads] stretches to go through
+  int* s_open = (int*)(s_at + cap);                                 // [threads, at least 192] stretches to go through
   __shared__ int s_n, s_left;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, waves = threads >> 6;
@@ -402,9 +410,9 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
         best = key > best ? key : best;
       }
     } else {
-      for (int i = tid; i < total * keep; i += threads) {
+      for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {   // (the product is below 2^31, the sum may pass it)
         const int g = cs_div(i, a.by_keep);
-        if (i - g * keep < stat[g].n) {
+        if ((int)i - g * keep < stat[g].n) {
           const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
           best = key > best ? key : best;
         }
@@ -474,14 +482,57 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   };
   const int n = s_n;
   if (n <= cap) {
-    for (int i = tid; i < n; i += threads) {
-      const uint64_t key = s_key[i];
-      const int64_t at = s_at[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += s_key[j] > key || (s_key[j] == key && s_at[j] < at);
-      if (rank < W) put(rank, key, at);
+    // ranks by counting: each candidate against all.  Where there are many (W above 32), those from a bound on that W to 128
+    // more reach, bisected: 600 candidates against all took one wavefront 390 us
+    int left = n;
+    if (n > 2 * W + 128) {
+      uint64_t most = 0;
+      for (int i = tid; i < n; i += threads) most = s_key[i] > most ? s_key[i] : most;
+      for (int o = 32; o; o >>= 1) {
+        const uint64_t u = __shfl_xor((unsigned long long)most, o);
+        most = u > most ? u : most;
+      }
+      __syncthreads();
+      if (lane == 0) s_wave[wave] = most;
+      __syncthreads();
+      for (int w = 0; w < waves; ++w) most = s_wave[w] > most ? s_wave[w] : most;
+      uint64_t lo = t, hi = most + 1;              // W or more reach lo, none hi
+      while (left > W + 128 && hi - lo > 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        __syncthreads();
+        if (tid == 0) s_left = 0;
+        __syncthreads();
+        int reach = 0;
+        for (int i = tid; i < n; i += threads) reach += s_key[i] >= mid;
+        for (int o = 32; o; o >>= 1) reach += __shfl_xor(reach, o);
+        if (lane == 0) atomicAdd(&s_left, reach);
+        __syncthreads();
+        if (s_left < W) hi = mid;
+        else { lo = mid; left = s_left; }
+      }
+      __syncthreads();
+      if (tid == 0) s_left = 0;
+      __syncthreads();
+      if (left <= W + 128)                         // (else that many are equal: all stay)
+        for (int i = tid; i < n; i += threads)
+          if (s_key[i] >= lo) s_open[atomicAdd(&s_left, 1)] = i;
+      __syncthreads();
     }
+    auto rank = [&](int m, auto place) {
+      for (int i = tid; i < m; i += threads) {
+        const uint64_t key = s_key[place(i)];
+        const int64_t at = s_at[place(i)];
+        int before = 0;
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) {
+          const uint64_t other = s_key[place(j)];
+          before += other > key || (other == key && s_at[place(j)] < at);
+        }
+        if (before < W) put(before, key, at);
+      }
+    };
+    if (left < n && left <= W + 128) rank(left, [&](int i) { return s_open[i]; });
+    else rank(n, [](int i) { return i; });
     for (int w = n + tid; w < W; w += threads) put(w, 0, 0);
     return;
   }
@@ -491,9 +542,9 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   for (int w = 0; w < W; ++w) {
     uint64_t key = 0;
     int64_t at = 0;
-    for (int i = tid; i < total * keep; i += threads) {
+    for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {
       const int g = cs_div(i, a.by_keep);
-      if (i - g * keep >= stat[g].n) continue;
+      if ((int)i - g * keep >= stat[g].n) continue;
       const uint64_t u = key_of(item[i].x, g);
       const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item[i].v;
       if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
@@ -591,15 +642,20 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   else launch_scan<_Float16>(a, grid, st);
   CS_HIP(hipGetLastError());
   // a wavefront per beam and a thread per stretch, as far as that goes
-  int64_t waves = ((int64_t)c->K * a.stretches + 63) / 64;
+  const int64_t total = (int64_t)c->K * a.stretches;
+  int64_t waves = (total + 63) / 64;
   waves = waves > c->K ? waves : c->K;
+  // (and for wide searches a thread for every 8 of some W candidates per stretch, so that the W-th largest of the threads' best
+  // is a good bound)
+  const int64_t wide = (total * c->W + 511) / 512;
+  waves = c->W > 32 && wide > waves ? wide : waves;
   const int threads = 64 * (int)(waves < BM_JOIN / 64 ? waves : BM_JOIN / 64);
   // places for what reaches the joined bound
   const int least = threads == 64 ? 128 : 1024;
   int cap = c->W * 32;
   cap = cap < least ? least : cap > 2048 ? 2048 : cap;
   hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads),
-                     (size_t)(((c->K * 8 + 15) & ~15) + cap * 16 + threads * 4), st, a, cap);
+                     (size_t)(((c->K * 8 + 15) & ~15) + cap * 16 + (threads < 192 ? 192 : threads) * 4), st, a, cap);
   CS_HIP(hipGetLastError());
   return CS_OK;
 }

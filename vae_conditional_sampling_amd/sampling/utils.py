@@ -299,13 +299,15 @@ class QuantisedHistory:
             out = torch.empty(shape, dtype=dtype, device=self._data.device)
             return out, kind, out.stride()
         kind, strides = _lib.CS_TYPE.get(out.dtype, 3), out.stride()
-        if out.shape != shape or kind == 3 or (strides[-1] != 1 and shape[-1] > 1):
-            raise _lib.CsError(f"out must be float32, bfloat16 or float16 {list(shape)} with adjacent values")
+        if out.shape != shape or kind == 3 or (strides[-1] != 1 and shape[-1] > 1) \
+                or any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+            raise _lib.CsError(f"out must be float32, bfloat16 or float16 {list(shape)} with adjacent values, every row a place "
+                               "of its own")
         return out, kind, strides
 
     def reorder(self, parents, steps=None):
-        """The records of every chain follow ``parents`` [B,K] in place (``beam.reorder_states``), in the first ``steps`` slots
-        (None: all)."""
+        """The records of every chain follow ``parents`` [B,K] in place (``beam.reorder_states``: K <= 64), in the first ``steps``
+        slots (None: all)."""
         from .beam import reorder_states
         data = self._data if steps is None else self._data[:int(steps)]
         reorder_states(data, parents, batch_dim=1, out=data)
