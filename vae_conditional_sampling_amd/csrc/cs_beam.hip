@@ -161,8 +161,8 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
   return t;
 }
 
-// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 628 of them for 2048 values, 352 of
-// these the 64-bit exponentials (11 each); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 us, 81 % of them issuing, where
+// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 628 of them for 2048 values, 328 of
+// these the 64-bit exponentials (82 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 us, 81 % of them issuing, where
 // their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the
 // next stretch before working on one (a fixed set of wavefronts) measured 141: twice the registers.
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
     t = bm_value(lo);
     const bool equal = c > keep;       // none found: lo is the W-th largest value, and others equal it
     n = 0;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // other lanes stored to these places above
 #pragma unroll
     for (int i = 0; i < LANE; ++i) {
       const bool take = equal ? x[i] > t : x[i] >= t;
@@ -318,28 +319,27 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
       if (take) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
       n += __popcll(m);
     }
-    if (equal) {
-    // of those equal to it the first ones
+    if (equal) {   // of those equal to it the first ones
 #pragma unroll
-    for (int j = 0; j < LANE / N; ++j) {
-      int mine = 0;
+      for (int j = 0; j < LANE / N; ++j) {
+        int mine = 0;
 #pragma unroll
-      for (int e = 0; e < N; ++e) mine += x[j * N + e] == t;
-      int incl = mine;
-      for (int o = 1; o < 64; o <<= 1) {
-        const int other = __shfl_up(incl, o);
-        if (lane >= o) incl += other;
-      }
-      int at = n + incl - mine;
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (x[j * N + e] == t) {
-          if (at < W) out[at] = BmItem{t, v_lane + j * 64 * N + e};
-          ++at;
+        for (int e = 0; e < N; ++e) mine += x[j * N + e] == t;
+        int incl = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+          const int other = __shfl_up(incl, o);
+          if (lane >= o) incl += other;
         }
-      n += __shfl(incl, 63);
-    }
-    n = n < W ? n : W;
+        int at = n + incl - mine;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (x[j * N + e] == t) {
+            if (at < W) out[at] = BmItem{t, v_lane + j * 64 * N + e};
+            ++at;
+          }
+        n += __shfl(incl, 63);
+      }
+      n = n < W ? n : W;
     }
   }
   if (lane == 0) a.stat[item] = BmStat{ref, sum, top, n};
@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     __syncthreads();
     uint32_t t32 = 1;
     for (int w = 0; w < waves; ++w) t32 = s_wave[w] > t32 ? (uint32_t)s_wave[w] : t32;
-    // where many of the lanes' best are left, the W-th largest of these (4 us; ranking the hundreds of candidates that are above the first bound took 10)
+    // where many of the lanes' best are left, the W-th largest of these (4 us; ranking the hundreds of candidates that are above
+    // the first bound took 10)
     const uint64_t reach = __ballot(best >= t32);
     if (waves > 1) {
       if (lane == 0) atomicAdd(&s_left, __popcll(reach));
@@ -576,8 +577,8 @@ int32_t stretches_of(const cs_beam_cfg& c) {
   const int64_t len = 64 * lane_values(c);
   return (int32_t)((c.V + len - 1) / len);
 }
-// logits kept of a stretch: what lies above the W-th largest of its lanes' best is a few more than W for W <= 32; for more, the
-// few best lanes no longer tell the best values, and the exact W are found
+// places for the logits kept of a stretch: what lies above the W-th largest of its lanes' best is a few more than W for
+// W <= 32; for more, nearly all lanes count, their best tell little, and a better bound is bisected
 int32_t keep_of(const cs_beam_cfg& c) { return c.W <= 32 ? 2 * c.W + 32 : 96; }
 
 template <typename T>
