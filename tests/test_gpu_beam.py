@@ -289,3 +289,26 @@ def test_wide_searches(B, K, V, W):
     check(beam_select(scores, logits, W), scores, logits, W)
     rows = logits.round()                                                                # (a dozen distinct ones)
     check(beam_select(scores, rows, W), scores, rows, W)
+
+
+def test_two_hundred_million_values():
+    V = 200_000_001
+    logits = torch.zeros(1, 1, V, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([V - 1, 0, 123_456_789, 2047, 2048, 99_999_999])
+    value = torch.tensor([3.0, 9.0, 5.0, 5.0, 12.0, 0.5])
+    logits[0, 0, at.cuda()] = value.bfloat16().cuda()
+    lse = float(np.log((V - 6) + np.exp(value.double().numpy()).sum()))
+    step = beam_select(torch.zeros(1, 1, dtype=torch.float64, device="cuda"), logits, 8)
+    want = [2048, 0, 2047, 123_456_789, V - 1, 99_999_999, 1, 2]      # (then the first of the zeros)
+    assert step.tokens[0].tolist() == want and not step.parents.any()
+    got = step.scores[0].cpu().numpy() + lse
+    assert np.allclose(got, [12.0, 9.0, 5.0, 5.0, 3.0, 0.5, 0.0, 0.0], rtol=0, atol=1e-9)
+
+
+def test_in_place_with_examples_outermost_in_memory():
+    g = torch.Generator().manual_seed(14)
+    big = torch.randn(5, 6, 7, 12, generator=g).cuda()
+    p = torch.randint(0, 7, (6, 7), generator=g).cuda()
+    apart = big.transpose(0, 1).contiguous().transpose(0, 1)
+    reorder_states(apart, p, batch_dim=1, out=apart)
+    assert torch.equal(apart.cpu(), torch.from_numpy(O.reorder(big.cpu().numpy(), p.cpu().numpy())))

@@ -98,3 +98,36 @@ def test_the_proposals_of_the_largest_weights(model, n):  # noqa: F811
     a, _ = run_sampler(S, model, X, M, **kw)
     b, _ = run_sampler(S, model, X, M, resample_final_imps_method="multinomial", **kw)
     assert torch.equal(a.final_resampling(X[:, 0].cpu(), M)[2], b.final_resampling(X[:, 0].cpu(), M)[2])
+
+
+def test_both_options_through_the_yaml_driver(tmp_path):
+    """top: the whole run and two shards of it write the same; the history in 8 bits: the run ends and keeps what is
+    observed."""
+    import os
+    from tests.helpers import ROOT
+    from vae_conditional_sampling_amd import distributed, driver
+    common = ["data.synthetic_num_test=90", "data.num_first_datapoints_test=61", "data.batch_size=32",
+              "test_class.init_args.num_iterations=12"]
+    top = common + ["test_class.init_args.resample_final_imps_method=top"]
+    load = lambda name, extra, root: driver.load_config(os.path.join(ROOT, name), extra + [f"trainer.default_root_dir={root}"])
+    name = "configs/uci_hepmass/sampling_u50/lair_k16_dmis_gr_mult_1replenish_wholedataset.yaml"
+    whole, _ = driver.run(load(name, top, tmp_path / "one"))
+    shards = [driver.run(load(name, top, tmp_path / "two"), rank=r, world_size=2)[0].collector.shard_arrays() for r in range(2)]
+    out = str(tmp_path / "two" / "merged")
+    distributed.write_batches(distributed.merge_shards(shards), 32, out)
+    files = [n for n in os.listdir(whole.out_dir) if n.startswith("irwg_imputations_after_final_resampling_")]
+    assert len(files) == 2
+    for n in files:
+        a, b = np.load(os.path.join(whole.out_dir, n)), np.load(os.path.join(out, n))
+        assert a["imputations"].shape[2] == 5 and all(np.array_equal(a[k], b[k]) for k in a.files)
+        m = np.broadcast_to(a["masks"][None], a["imputations"].shape)
+        assert np.array_equal(a["imputations"][m], np.broadcast_to(a["true_X"][None], m.shape)[m])
+    name = "configs/uci_miniboone/sampling_u50/lair_k4_dmis_gr_mult_1replenish.yaml"
+    past = common + ["test_class.init_args.resample_final_imps=False", "test_class.init_args.num_historical_proposals=2",
+                     "test_class.init_args.no_historic_proposals_iterations=3", "test_class.init_args.imputation_history_length=6",
+                     "test_class.init_args.imputation_history_format=int8"]
+    tester, outs = driver.run(load(name, past, tmp_path / "past"))
+    f = np.load(os.path.join(tester.out_dir, "imputations_0.npz"))
+    m = np.broadcast_to(f["masks"][None], f["imputations"].shape)
+    assert np.isfinite(f["imputations"]).all()
+    assert np.array_equal(f["imputations"][m], np.broadcast_to(f["true_X"][None], m.shape)[m])
