@@ -499,7 +499,7 @@ typedef struct {
 } cs_beam_cfg;
 /* Bytes of device memory cs_beam_select needs as `workspace` (8-byte aligned), or -1 for a bad configuration. */
 int64_t cs_beam_select_workspace(const cs_beam_cfg* cfg);
-/* Per example the W largest s[k,v] = logits[k,v] + (scores[k] - lse[k]), descending, ties to the lowest k*V + v, where
+/* Per example the W largest s[k,v] = scores[k] + (logits[k,v] - lse[k]), descending, ties to the lowest k*V + v, where
  * lse[k] is the log of the sum of exponentials of beam k's allowed logits (0 with normalise = 0), all in 64 bits.
  *   scores[B,K] (NULL: zeros), logits[B,K,V], mask (NULL: all) 1 = allowed: what is not allowed is neither a candidate
  *   nor in the normaliser, whatever its logit holds; finished[B,K] (NULL: none): such a beam has one candidate,

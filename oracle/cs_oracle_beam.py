@@ -27,7 +27,7 @@ def beam_select(scores, logits, width, *, normalise=True, mask=None, finished=No
                     top = row.max()
                     lse = top + math.log(np.exp(row - top).sum())
                 with np.errstate(invalid="ignore"):
-                    s = row + (before - lse)
+                    s = before + (row - lse)
             v = np.flatnonzero(s > -np.inf)    # (a NaN is not)
             # (of one beam only the first W by (score, index) can be among the W best)
             v = v[np.lexsort((v, -s[v]))[:width]]

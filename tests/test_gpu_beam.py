@@ -312,3 +312,28 @@ def test_in_place_with_examples_outermost_in_memory():
     apart = big.transpose(0, 1).contiguous().transpose(0, 1)
     reorder_states(apart, p, batch_dim=1, out=apart)
     assert torch.equal(apart.cpu(), torch.from_numpy(O.reorder(big.cpu().numpy(), p.cpu().numpy())))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_beams_with_one_value_left_keep_their_score(dtype):
+    """A normaliser over one value is that value: the score stays what it was to the last bit, and equal beams keep their
+    order."""
+    g = torch.Generator().manual_seed(21)
+    for B, K, V in ((3, 7, 1), (2, 9, 500), (2, 5, 6000)):
+        logits = (torch.randn(B, K, V, generator=g) * 20).to(dtype).cuda()
+        keep = torch.randint(0, V, (B, K, 1), generator=g)
+        mask = torch.zeros(B, K, V, dtype=torch.bool).scatter_(2, keep, True).cuda()
+        for scores in (torch.zeros(B, K, dtype=torch.float64), torch.randn(B, K, generator=g).double().mul(4).round() / 3):
+            step = beam_select(scores.cuda(), logits, K, mask=mask)
+            order = torch.sort(scores, dim=1, descending=True, stable=True)
+            assert torch.equal(step.scores.cpu(), order.values) and torch.equal(step.parents.cpu(), order.indices)
+            assert torch.equal(step.tokens.cpu(), keep[:, :, 0].gather(1, order.indices))
+    # all but certain beams: what is left of the probability tells them apart
+    sure = torch.zeros(1, 6, 3000, dtype=dtype)
+    for k, gap in enumerate((24.0, 30.0, 27.0, 33.0, 26.0, 21.0)):
+        sure[0, k, :] = -gap
+        sure[0, k, 17 * k] = 0.0
+    step = beam_select(None, sure.cuda(), 6)
+    assert step.parents[0].tolist() == [3, 1, 2, 4, 0, 5]
+    want = -np.log1p(2999 * np.exp(-np.array([33.0, 30, 27, 26, 24, 21])))
+    assert np.allclose(host(step.scores)[0], want, rtol=1e-4, atol=0)

@@ -1,7 +1,7 @@
 // Beam search over chains: the best continuations of all beams of an example, and the states that follow them.  The
 // deterministic sibling of the multinomial / systematic resampling (cs_lair.hip, cs_final_resample).
 //
-// Selection.  s[k,v] = logits[k,v] + (scores[k] - lse[k]), lse the log of the sum of exponentials of the allowed logits
+// Selection.  s[k,v] = scores[k] + (logits[k,v] - lse[k]), lse the log of the sum of exponentials of the allowed logits
 // of beam k: the W largest over (k,v), ties to the lowest k*V + v.  One pass over the logits: a wavefront holds a
 // stretch of one beam in registers (LANE values per lane), leaves their sum of exponentials and those of them that can
 // be among its W best in the workspace; a workgroup per example then joins the stretches of every beam, turns the
@@ -126,9 +126,10 @@ __device__ const double bm_pow64[64] = {
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509};
 
 // exp(d) for |d| <= 690 as 2^n 2^(j/64) exp(r), 64 n + j the integer nearest to 64 d / ln 2 and |r| <= ln 2 / 128, exp(r) by its
-// Taylor polynomial of degree 3 (remainder r^4 / 24 < 3.6e-11): the table-driven method of Tang (1989).  Adding 1.5 * 2^52
+// Taylor polynomial of degree 4 (remainder r^5 / 120 < 4e-14; degree 3, 3.6e-11, would be 3 us faster on the largest case and
+// mistakes the order of beams that are certain to 1e-11): the table-driven method of Tang (1989).  Adding 1.5 * 2^52
 // leaves the integer in the low word.  The table lies in the lanes' registers and is read by ds_bpermute, which takes the
-// lane from the index's low 6 bits by itself; its high words have j << 14 taken off beforehand, so one shift and addition of
+// lane (all of them have to be there) from the index's low 6 bits by itself; its high words have j << 14 taken off beforehand, so one shift and addition of
 // the whole integer puts the exponent right.
 struct BmPow {
   int hi, lo;
@@ -144,7 +145,7 @@ __device__ __forceinline__ double bm_add_exp(double sum, double d, const BmPow& 
   const int nj = __double2loint(z);
   const double r = __builtin_fma(z - MAGIC, -0.010830424696249145, d);
   const int hi = __builtin_amdgcn_ds_bpermute(nj << 2, pow.hi) + (nj << 14), lo = __builtin_amdgcn_ds_bpermute(nj << 2, pow.lo);
-  const double p = __builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 6, 0.5), r, 1.0), r, 1.0);
+  const double p = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
   return __builtin_fma(__hiloint2double(hi, lo), p, sum);
 }
 
@@ -161,8 +162,8 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
   return t;
 }
 
-// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 628 of them for 2048 values, 328 of
-// these the 64-bit exponentials (82 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 us, 81 % of them issuing, where
+// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 660 of them for 2048 values, 360 of
+// these the 64-bit exponentials (90 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 us, 81 % of them issuing, where
 // their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the
 // next stretch before working on one (a fixed set of wavefronts) measured 141: twice the registers.
@@ -349,8 +350,9 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
 // 64, 10.7 for 4096 examples of 5 stretches.
 __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, int cap) {
   extern __shared__ char lds[];
-  double* s_beam = (double*)lds;                                    // [K] what a kept logit of the beam gets added
-  uint64_t* s_key = (uint64_t*)(lds + ((a.c.K * 8 + 15) & ~15));    // [cap] scores of candidates, as ordered bits
+  double* s_lse = (double*)lds;                                     // [K]
+  double* s_before = s_lse + a.c.K;                                 // [K] scores
+  uint64_t* s_key = (uint64_t*)(s_before + a.c.K);                  // [cap] scores of candidates, as ordered bits
   int64_t* s_at = (int64_t*)(s_key + cap);                          // [cap] k << 32 | v
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
@@ -368,35 +370,58 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   const float top0 = tid < total ? stat[tid].top : -__builtin_inff();
   const int n0 = tid < total ? stat[tid].n : 0;
   const int n_first = total <= 64 && lane < total ? stat[lane].n : 0;
+  const BmPow pow(lane);
   if (tid == 0) { s_n = 0; s_left = 0; }
   for (int k = wave; k < K; k += waves) {
     const int64_t row = b * K + k;
-    double before = 0.0;
+    double before = 0.0, lse = 0.0;
     if (a.scores) before = a.c.scores_type == CS_TYPE_F64 ? ((const double*)a.scores)[row] : (double)((const float*)a.scores)[row];
     if (a.c.normalise && !(a.finished && a.finished[row])) {
       const BmStat* st = stat + k * C;
-      // lanes join their stretches, then each other
-      double ref = -INF, sum = 0.0;
+      // Lanes join their stretches, then each other: those of reference 0 (the rule) and, apart, the others.
+      float top = -__builtin_inff();               // of the former
+      double sum = 0.0, ref = -INF, far = 0.0;     // far: of the latter, relative to ref
       for (int c = lane; c < C; c += 64) {
         const BmStat s = st[c];
         if (s.sum != s.sum) sum = s.sum;             // (NaN stays)
         if (!(s.top > -__builtin_inff())) continue;  // nothing allowed there
-        const double m = fmax(ref, s.ref);
-        sum = sum * (ref == m ? 1.0 : exp(ref - m)) + s.sum * (s.ref == m ? 1.0 : exp(s.ref - m));
-        ref = m;
+        if (s.ref == 0.0) {
+          top = fmaxf(top, s.top);
+          sum += s.sum;
+        } else {
+          const double m = fmax(ref, s.ref);
+          far = far * exp(ref - m) + s.sum * exp(s.ref - m);
+          ref = m;
+        }
       }
-      double m = 0.0;                  // (the rule: all values within their bounds, so all of reference 0)
-      if (__ballot(ref != 0.0 && ref > -INF) || !__ballot(ref == 0.0)) {
-        m = ref;
-        for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+      top = bm_wave_max(top);
+      sum = bm_wave_sum(sum);
+      double m = (double)top;
+      if (__ballot(ref > -INF)) {
+        double all = ref;
+        for (int o = 32; o; o >>= 1) all = fmax(all, __shfl_xor(all, o));
+        far = bm_wave_sum(ref > -INF ? far * exp(ref - all) : far);
+        ref = all;
+        m = fmax(m, ref);
+        far *= exp(ref - m);
       }
-      sum = bm_wave_sum(ref > -INF && ref != m ? sum * exp(ref - m) : sum);
-      before -= m + log(sum);          // (+inf, NaN or nothing allowed: NaN or +inf, with no candidate left to count)
+      // The sum relative to the largest logit, that logit's own part being one exactly: a beam left with one value has a
+      // normaliser of just its logit, and of a beam that is all but certain the rest counts, not the roundings of the whole.
+      if (m == (double)top && top > -__builtin_inff()) {
+        const double e = bm_add_exp(0.0, m, pow);
+        sum = 1.0 + (sum - e) / e;
+      } else if (top > -__builtin_inff()) {
+        sum *= exp(-m);
+      }
+      lse = m + log(sum + far);        // (+inf, NaN or nothing allowed: NaN or -inf, with no candidate left to count)
     }
-    if (lane == 0) s_beam[k] = before;
+    if (lane == 0) { s_lse[k] = lse; s_before[k] = before; }
   }
   __syncthreads();
-  auto key_of = [&](float x, int g) { return bm_key64((double)x + s_beam[cs_div(g, a.by_stretches)]); };
+  auto key_of = [&](float x, int g) {   // (in this order: where x is the whole normaliser, the score stays what it was)
+    const uint32_t k = cs_div(g, a.by_stretches);
+    return bm_key64(s_before[k] + ((double)x - s_lse[k]));
+  };
   // a bound from below; none where there are few candidates
   uint64_t t = 1;
   if (total > 64 || bm_wave_sum((double)n_first) > cap / 2) {
@@ -652,11 +677,11 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   waves = c->W > 32 && wide > waves ? wide : waves;
   const int threads = 64 * (int)(waves < BM_JOIN / 64 ? waves : BM_JOIN / 64);
   // places for what reaches the joined bound
-  const int least = threads == 64 ? 128 : 1024;
+  const int least = threads == 64 ? 128 : 1024, most = c->K > 1024 ? 1024 : 2048;   // (64 KB of LDS in all)
   int cap = c->W * 32;
-  cap = cap < least ? least : cap > 2048 ? 2048 : cap;
+  cap = cap > most ? most : cap < least ? least : cap;
   hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads),
-                     (size_t)(((c->K * 8 + 15) & ~15) + cap * 16 + (threads < 192 ? 192 : threads) * 4), st, a, cap);
+                     (size_t)(c->K * 16 + cap * 16 + (threads < 192 ? 192 : threads) * 4), st, a, cap);
   CS_HIP(hipGetLastError());
   return CS_OK;
 }

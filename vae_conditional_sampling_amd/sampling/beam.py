@@ -50,7 +50,7 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
     ``scores`` [B,K] float32 / float64 (None: zeros, float32): what the beams have so far; -inf: a beam that is not in use (the
     first step of a search starts from one beam).  ``logits`` [B,K,V] float32 / bfloat16 / float16, the values adjacent in
     memory, any strides of the other axes.  A continuation scores
-    ``scores + logits - logsumexp(logits)``, or ``scores + logits`` with ``normalise=False``, formed in 64 bits;
+    ``scores + (logits - logsumexp(logits))``, or ``scores + logits`` with ``normalise=False``, formed in 64 bits;
     equal scores go to the lowest (beam, value).  ``mask`` (bool, broadcastable to [B,K,V]; True = allowed): what is not
     allowed takes no part in the normaliser either and may hold anything.  ``finished`` [B,K] (bool): such a beam only
     continues with ``end_token``, at its score; its logits are not read.  NaN and -inf are never chosen; a beam with a NaN or
