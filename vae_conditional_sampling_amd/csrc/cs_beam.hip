@@ -19,7 +19,6 @@ constexpr int BM_MAXK = 2048;
 constexpr int BM_JOIN = 1024;          // threads that join an example, at most
 constexpr float BM_LOWEST = -3.402823466e+38f;
 
-struct BmItem { float x; int32_t v; };
 // of a stretch: the sum of exp(x - ref), the largest logit, the number of kept ones
 struct BmStat { double ref, sum; float top; int32_t n; };
 
@@ -28,7 +27,8 @@ struct BmArgs {
   const void *scores, *logits;
   const uint8_t *mask, *finished;
   BmStat* stat;     // [B*K*stretches]
-  BmItem* item;     // [B*K*stretches][keep]
+  float* item_x;    // [B*K*stretches][keep] the logits kept of a stretch
+  int32_t* item_v;  // and their values
   void* out_scores;
   int64_t *parents, *tokens;
   int32_t stretches, keep;
@@ -162,9 +162,10 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
   return t;
 }
 
-// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 660 of them for 2048 values, 360 of
-// these the 64-bit exponentials (90 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 us, 81 % of them issuing, where
-// their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
+// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 654 of them for 2048 values, 364 of
+// these the 64-bit exponentials (91 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 to 92 us, 85 % of
+// them issuing, where their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
+// (Logits and values kept in two arrays, so that a kept one costs 4 instructions and not 8: 3 % faster.)
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the
 // next stretch before working on one (a fixed set of wavefronts) measured 141: twice the registers.
 template <typename T, bool MASK, int LANE>
@@ -179,11 +180,12 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   const uint32_t b = cs_div(row, a.by_K), k = row - b * a.c.K;
   const int W = a.c.W, keep = a.keep;
   const int32_t V = (int32_t)a.c.V;
-  BmItem* out = a.item + (int64_t)item * keep;
+  float* out_x = a.item_x + (int64_t)item * keep;
+  int32_t* out_v = a.item_v + (int64_t)item * keep;
   if (a.finished && a.finished[row]) {   // its one candidate keeps the beam's score; its logits are not read
     if (lane == 0) {
       a.stat[item] = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
-      if (base == 0) out[0] = BmItem{0.0f, (int32_t)a.c.end_token};
+      if (base == 0) { out_x[0] = 0.0f; out_v[0] = (int32_t)a.c.end_token; }
     }
     return;
   }
@@ -290,9 +292,13 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   for (int i = 0; i < LANE; ++i) {
     const uint64_t m = __ballot(x[i] >= t);
     if (m) {
-      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
-      n += __popcll(m);
-      if (n <= keep && x[i] >= t) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
+      const int c = __popcll(m);
+      if (n + c <= keep && x[i] >= t) {
+        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        (out_x + n)[at] = x[i];
+        (out_v + n)[at] = v_lane + (i / N) * 64 * N + i % N;
+      }
+      n += c;
     }
   }
   if (n > keep) {
@@ -316,8 +322,11 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
     for (int i = 0; i < LANE; ++i) {
       const bool take = equal ? x[i] > t : x[i] >= t;
       const uint64_t m = __ballot(take);
-      const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, n));
-      if (take) out[at] = BmItem{x[i], v_lane + (i / N) * 64 * N + i % N};
+      const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      if (take) {
+        (out_x + n)[at] = x[i];
+        (out_v + n)[at] = v_lane + (i / N) * 64 * N + i % N;
+      }
       n += __popcll(m);
     }
     if (equal) {   // of those equal to it the first ones
@@ -335,7 +344,7 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
 #pragma unroll
         for (int e = 0; e < N; ++e)
           if (x[j * N + e] == t) {
-            if (at < W) out[at] = BmItem{t, v_lane + j * 64 * N + e};
+            if (at < W) { out_x[at] = t; out_v[at] = v_lane + j * 64 * N + e; }
             ++at;
           }
         n += __shfl(incl, 63);
@@ -346,8 +355,8 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   if (lane == 0) a.stat[item] = BmStat{ref, sum, top, n};
 }
 
-// One workgroup per example; bound by its chain of dependent loads and barriers: 5.4 us for 4 beams of 32 stretches, 15 for 16 of
-// 64, 10.7 for 4096 examples of 5 stretches.
+// One workgroup per example; bound by its chain of dependent loads and barriers: 5.9 us for 4 beams of 32 stretches, 16 for 16 of
+// 64, 12 for 4096 examples of 5 stretches.
 __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, int cap) {
   extern __shared__ char lds[];
   double* s_lse = (double*)lds;                                     // [K]
@@ -364,7 +373,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
   const int32_t total = K * C;         // (at most 2^31 / keep, checked on the host)
   const BmStat* stat = a.stat + b * total;
-  const BmItem* item = a.item + b * total * keep;
+  const float* item_x = a.item_x + b * total * keep;
+  const int32_t* item_v = a.item_v + b * total * keep;
   constexpr double INF = __builtin_inf();
   // (asked for before the normalisers are formed)
   const float top0 = tid < total ? stat[tid].top : -__builtin_inff();
@@ -438,7 +448,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
       for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {   // (the product is below 2^31, the sum may pass it)
         const int g = cs_div(i, a.by_keep);
         if ((int)i - g * keep < stat[g].n) {
-          const uint32_t key = (uint32_t)(key_of(item[i].x, g) >> 32);
+          const uint32_t key = (uint32_t)(key_of(item_x[i], g) >> 32);
           best = key > best ? key : best;
         }
       }
@@ -489,11 +499,11 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     for (int o = tid >> 4; o < open; o += threads >> 4) {
       const int h = s_open[o], n = g0 == 0 && h == tid ? n0 : stat[h].n;
       for (int r = tid & 15; r < n; r += 16) {
-        const BmItem i = item[(int64_t)h * keep + r];
-        const uint64_t key = key_of(i.x, h);
+        const int64_t i = (int64_t)h * keep + r;
+        const uint64_t key = key_of(item_x[i], h);
         if (key < t) continue;
         const int at = atomicAdd(&s_n, 1);   // (places in any order: the ranks below depend on the entries alone)
-        if (at < cap) { s_key[at] = key; s_at[at] = (int64_t)cs_div(h, a.by_stretches) << 32 | i.v; }
+        if (at < cap) { s_key[at] = key; s_at[at] = (int64_t)cs_div(h, a.by_stretches) << 32 | item_v[i]; }
       }
     }
   }
@@ -571,8 +581,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
     for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {
       const int g = cs_div(i, a.by_keep);
       if ((int)i - g * keep >= stat[g].n) continue;
-      const uint64_t u = key_of(item[i].x, g);
-      const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item[i].v;
+      const uint64_t u = key_of(item_x[i], g);
+      const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item_v[i];
       if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
     }
     for (int o = 32; o; o >>= 1) {
@@ -636,7 +646,7 @@ int check_beam(const cs_beam_cfg* c) {
 
 extern "C" int64_t cs_beam_select_workspace(const cs_beam_cfg* c) {
   if (check_beam(c)) return -1;
-  return (int64_t)c->B * c->K * stretches_of(*c) * (int64_t)(sizeof(BmStat) + keep_of(*c) * sizeof(BmItem));
+  return (int64_t)c->B * c->K * stretches_of(*c) * (int64_t)(sizeof(BmStat) + keep_of(*c) * 8);
 }
 
 extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const void* logits, const uint8_t* mask,
@@ -655,7 +665,8 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   a.keep = keep_of(*c);
   const int64_t items = (int64_t)c->B * c->K * a.stretches;
   a.stat = (BmStat*)workspace;
-  a.item = (BmItem*)(a.stat + items);
+  a.item_x = (float*)(a.stat + items);
+  a.item_v = (int32_t*)(a.item_x + items * a.keep);
   a.out_scores = out_scores; a.parents = parents; a.tokens = tokens;
   hipStream_t st = (hipStream_t)stream;
   a.items = (uint32_t)items;
