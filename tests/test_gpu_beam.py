@@ -1,6 +1,8 @@
 """beam_select and reorder_states against plain forms in float64 (oracle/cs_oracle_beam.py).  Indices are exact; a score is
 the 64-bit value rounded once, off by at most half a step of its type (2^-24 relative in float32); the kernel's 64-bit
 value itself is off by the summation of the normaliser: 1e-10 absolute covers 2^17 terms of relative error below 4e-11."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -337,3 +339,29 @@ def test_beams_with_one_value_left_keep_their_score(dtype):
     assert step.parents[0].tolist() == [3, 1, 2, 4, 0, 5]
     want = -np.log1p(2999 * np.exp(-np.array([33.0, 30, 27, 26, 24, 21])))
     assert np.allclose(host(step.scores)[0], want, rtol=1e-4, atol=0)
+
+
+def test_seventeen_million_examples():
+    """More threads than an axis of a launch may hold, in the selection's two kernels and in moving what follows.  The values of
+    an example differ by 1/8 and more, so float32 tells them apart."""
+    B, K, V = (1 << 24) + 5, 4, 4
+    v = torch.arange(B * K, device="cuda").reshape(B, K)
+    best = (v * 7 + v // 13) % V
+    logits = torch.zeros(B, K, V, dtype=torch.bfloat16, device="cuda")
+    logits.scatter_(2, best[..., None], 2.0)
+    scores = ((v * 5) % 4).float() * 0.125                                               # of K beams a permutation of 0, 1, 2, 3 eighths
+    got = beam_select(scores, logits, 1)
+    at = scores.argmax(1, keepdim=True)
+    assert torch.equal(got.parents, at)
+    assert torch.equal(got.tokens, best.gather(1, at))
+    want = 0.375 + 2.0 - math.log(math.exp(2.0) + 3)
+    assert float((got.scores.double() - want).abs().max()) <= 2.0 ** -24 * abs(want) + SUM
+    del logits, got
+    rows = torch.empty(B, 2, 257, dtype=torch.uint8, device="cuda")
+    tag = (v[:, :2] * 3 + 1).remainder(251).to(torch.uint8)[..., None]
+    rows.copy_(tag.expand_as(rows))
+    swap = torch.tensor([1, 0], device="cuda").expand(B, 2)
+    moved = reorder_states(rows, swap)
+    reorder_states(rows, swap, out=rows)
+    assert torch.equal(moved, rows)
+    assert bool((rows == tag.flip(1)).all())

@@ -337,3 +337,17 @@ def test_captured_step_replays_with_new_inputs():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, ref))
         assert torch.equal(q.data, e.data)
+
+
+def test_a_billion_states_in_one_call():
+    """More threads than an axis of a launch may hold.  Integers up to 100 beside a value of 127 have a scale of one in int8."""
+    B, K, D = 1 << 20, 1025, 2
+    q = QuantisedHistory(1, (B, K, D), "int8", group=32)
+    x = torch.full((B, K, D), 127, dtype=torch.float16, device="cuda")
+    x[..., 1] = (torch.arange(B * K, device="cuda") % 101).reshape(B, K)
+    q.write(x, 0)
+    back = q.read_steps(0, 1, dtype=torch.float16)
+    assert torch.equal(back[0], x)
+    at = torch.zeros(1, 1, 1, dtype=torch.int64, device="cuda").expand(1, B, K)
+    back.zero_()
+    assert torch.equal(q.read(at, out=back)[0], x)

@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
   constexpr int N = BmElem<T>::N;      // logits in 16 bytes
   constexpr float INF = __builtin_inff();
   const int lane = threadIdx.x & 63;
-  const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t item = cs_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= a.items) return;
   const uint32_t row = cs_div(item, a.by_stretches);
   const int32_t base = (int32_t)(item - row * a.stretches) * (64 * LANE);
@@ -369,7 +369,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   __shared__ int s_n, s_left;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, waves = threads >> 6;
-  const int64_t b = blockIdx.x;
+  const int64_t b = cs_block();
+  if (b >= a.c.B) return;
   const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
   const int32_t total = K * C;         // (at most 2^31 / keep, checked on the host)
   const BmStat* stat = a.stat + b * total;
@@ -673,7 +674,7 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   a.by_stretches = cs_div_by(a.stretches);
   a.by_K = cs_div_by(c->K);
   a.by_keep = cs_div_by(a.keep);
-  const dim3 grid((unsigned)((items + 3) / 4));
+  const dim3 grid = cs_grid((items + 3) / 4);
   if (c->logits_type == CS_TYPE_F32) launch_scan<float>(a, grid, st);
   else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, grid, st);
   else launch_scan<_Float16>(a, grid, st);
@@ -691,7 +692,7 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   const int least = threads == 64 ? 128 : 1024, most = c->K > 1024 ? 1024 : 2048;   // (64 KB of LDS in all)
   int cap = c->W * 32;
   cap = cap > most ? most : cap < least ? least : cap;
-  hipLaunchKernelGGL(cs_beam_join_kernel, dim3((unsigned)c->B), dim3(threads),
+  hipLaunchKernelGGL(cs_beam_join_kernel, cs_grid(c->B), dim3(threads),
                      (size_t)(c->K * 16 + cap * 16 + (threads < 192 ? 192 : threads) * 4), st, a, cap);
   CS_HIP(hipGetLastError());
   return CS_OK;
@@ -716,7 +717,7 @@ struct BmMoveArgs {
 // out of place: a thread per vector of a destination row, over its outer indices
 template <typename VEC>
 __global__ void __launch_bounds__(256) cs_beam_gather_kernel(const BmMoveArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)cs_block() * 256 + threadIdx.x;
   if (i >= a.B * a.W * a.cols) return;
   const int64_t bw = i / a.cols, col = i - bw * a.cols;
   const int64_t p = a.parents[bw];
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(256) cs_beam_gather_kernel(const BmMoveArgs a)
   const int64_t b = bw / a.W, w = bw - b * a.W;
   const char* s = a.src + b * a.ss[1] + p * a.ss[2] + col * sizeof(VEC);
   char* d = a.dst + b * a.ds[1] + w * a.ds[2] + col * sizeof(VEC);
-  for (int64_t o = blockIdx.y; o < a.outer; o += a.outer_step)
+  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step)
     *(VEC*)(d + o * a.ds[0]) = *(const VEC*)(s + o * a.ss[0]);
 }
 
@@ -735,7 +736,7 @@ __global__ void __launch_bounds__(256) cs_beam_gather_kernel(const BmMoveArgs a)
 // with several columns a lane 86, streaming stores and loads 93 and 107.)
 template <typename VEC, int KMAX>
 __global__ void __launch_bounds__(256) cs_beam_inplace_kernel(const BmMoveArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)cs_block() * 256 + threadIdx.x;
   if (i >= a.B * a.cols) return;
   const int64_t b = i / a.cols, col = i - b * a.cols;
   int parent[KMAX];
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(256) cs_beam_inplace_kernel(const BmMoveArgs a
     parent[k] = p < 0 || p >= a.K || p == k ? -1 : (int)p;
   }
   char* d = a.dst + b * a.ds[1] + col * sizeof(VEC);
-  for (int64_t o = blockIdx.y; o < a.outer; o += a.outer_step) {
+  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step) {
     VEC v[KMAX];
 #pragma unroll
     for (int k = 0; k < KMAX; ++k)
@@ -816,7 +817,8 @@ extern "C" int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_
   split = split < 1 ? 1 : split;
   split = split < outer ? split : outer;
   a.outer_step = split < 65535 ? split : 65535;
-  const dim3 grid((unsigned)blocks, (unsigned)a.outer_step);
+  dim3 grid = cs_grid(blocks);
+  grid.z = (unsigned)a.outer_step;
   hipStream_t st = (hipStream_t)stream;
   if (vec == 16) launch_move<u32x4>(a, in_place, grid, st);
   else if (vec == 8) launch_move<u32x2>(a, in_place, grid, st);

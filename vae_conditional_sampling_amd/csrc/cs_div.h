@@ -1,5 +1,5 @@
 // n / d for any 32-bit n by a multiplication (the round-up form of Granlund and Montgomery, 1994), d from 1 to 2^32 - 1: a
-// 64-bit division by a size of the call costs a lane several hundred instructions, a 32-bit one about forty.
+// 64-bit division by a size of the call costs a lane several hundred instructions, a 32-bit one about forty.  And grids of more workgroups than a launch's first axis may hold.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -17,3 +17,12 @@ __device__ __forceinline__ uint32_t cs_div(uint32_t n, const CsDiv& d) {
   const uint32_t t = __umulhi(n, d.mul);
   return d.shift == 0 ? n : (t + ((n - t) >> 1)) >> (d.shift - 1);
 }
+
+// Workgroups of 256 to 1024 threads in two axes (an axis of a launch has to stay below 2^32 threads), and the number of one;
+// the last row may hold more workgroups than were asked for.  At most 2^36 of them.
+constexpr int CS_GRID_SHIFT = 20;
+inline dim3 cs_grid(int64_t blocks) {
+  constexpr int64_t ROW = 1ll << CS_GRID_SHIFT;
+  return blocks <= ROW ? dim3((unsigned)blocks) : dim3((unsigned)ROW, (unsigned)((blocks + ROW - 1) >> CS_GRID_SHIFT));
+}
+__device__ __forceinline__ uint32_t cs_block() { return (blockIdx.y << CS_GRID_SHIFT) + blockIdx.x; }

@@ -188,7 +188,7 @@ __device__ __forceinline__ void qc_store8(T* p, const float* v) {
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
   const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
-  const uint32_t row = blockIdx.x * (uint32_t)a.rows_per_block + (uint32_t)ry;
+  const uint32_t row = cs_block() * (uint32_t)a.rows_per_block + (uint32_t)ry;
   if (ry >= a.rows_per_block || row >= a.rows) return;
   const uint32_t i = cs_div(row, a.by_chains), chain = row - i * a.by_chains.d;
   const int32_t slot = qc_slot(a, i, chain);
@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
   extern __shared__ __align__(16) char lds[];
   T* s_out = (T*)lds;                  // [R * rows_per_block][D]
   const int ry = (int)cs_div(threadIdx.x, a.by_lanes);
-  const uint32_t row0 = blockIdx.x * (uint32_t)(R * a.rows_per_block);
+  const uint32_t row0 = cs_block() * (uint32_t)(R * a.rows_per_block);
+  if (row0 >= a.rows) return;
   const char* rec[R];
   T* out[R];
   bool live[R], there[R];
@@ -369,7 +370,7 @@ int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStr
   const bool packed = !WRITE && c.D % QC_LANE != 0 && a.lanes <= 16 && a.stride[2] == c.D && a.stride[1] == (int64_t)inner * c.D &&
                       (n == 1 || a.stride[0] == c.B * inner * c.D);
   const int R = WRITE || packed || blocks < 8192 ? 1 : 4;
-  const dim3 grid((blocks + R - 1) / R);
+  const dim3 grid = cs_grid((blocks + R - 1) / R);
   if (c.fmt == CS_QFMT_INT8) launch_type<WRITE, CS_QFMT_INT8>(a, type, R, packed, grid, st);
   else if (c.fmt == CS_QFMT_MXFP8) launch_type<WRITE, CS_QFMT_MXFP8>(a, type, R, packed, grid, st);
   else launch_type<WRITE, CS_QFMT_MXFP4>(a, type, R, packed, grid, st);
