@@ -365,3 +365,24 @@ def test_seventeen_million_examples():
     reorder_states(rows, swap, out=rows)
     assert torch.equal(moved, rows)
     assert bool((rows == tag.flip(1)).all())
+
+
+@pytest.mark.parametrize("kind", ["plain", "masked", "integers", "far"])
+@pytest.mark.parametrize("B,K,V,W", [(700, 1, 2000, 5), (9, 8, 512, 64), (5, 2, 2048, 33), (3, 1, 4096, 64), (1700, 4, 2047, 4),
+                                     (100, 8, 100, 64), (40, 3, 1030, 16), (300, 16, 33, 40), (1300, 1, 10200, 40), (1300, 1, 10200, 64),
+                                     (6, 13, 900, 7), (520, 2, 9000, 24)])
+def test_few_stretches_and_many_examples(B, K, V, W, kind):
+    """What one launch does, and what is joined by one wavefront or a few."""
+    scores, logits, g = make(B, K, V, torch.float32, B + V + W)
+    kw = {}
+    if kind == "masked":
+        kw = dict(mask=(torch.rand(B, 1, V, generator=g) < 0.4).cuda(), finished=(torch.rand(B, K, generator=g) < 0.3).cuda(),
+                  end_token=V // 2)
+    elif kind == "integers":      # hundreds of equal values
+        logits, scores = logits.round(), scores.round()
+        kw = dict(normalise=False)
+    elif kind == "far":           # normalisers relative to a stretch's largest value beside absolute ones, in some beams alone
+        logits[::3, 0] += 2000
+        logits[1::3, :, V // 2:] -= 900
+        logits[2::3, -1, : V // 3] = float("-inf")
+    check(beam_select(scores, logits, W, **kw), scores, logits, W, **kw)

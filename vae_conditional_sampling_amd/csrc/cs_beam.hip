@@ -17,6 +17,7 @@ namespace {
 constexpr int BM_MAXW = 64;            // candidates per example: a lane each
 constexpr int BM_MAXK = 2048;
 constexpr int BM_JOIN = 1024;          // threads that join an example, at most
+constexpr int BM_ONE = 8;              // stretches of an example, at most, for one launch that does it all
 constexpr float BM_LOWEST = -3.402823466e+38f;
 
 // of a stretch: the sum of exp(x - ref), the largest logit, the number of kept ones
@@ -169,22 +170,17 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the
 // next stretch before working on one (a fixed set of wavefronts) measured 141: twice the registers.
 template <typename T, bool MASK, int LANE>
-__global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
+__device__ __forceinline__ void bm_scan(const BmArgs& a, uint32_t row, uint32_t stretch, BmStat* stat, float* out_x, int32_t* out_v) {
   constexpr int N = BmElem<T>::N;      // logits in 16 bytes
   constexpr float INF = __builtin_inff();
   const int lane = threadIdx.x & 63;
-  const uint32_t item = cs_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= a.items) return;
-  const uint32_t row = cs_div(item, a.by_stretches);
-  const int32_t base = (int32_t)(item - row * a.stretches) * (64 * LANE);
+  const int32_t base = (int32_t)stretch * (64 * LANE);
   const uint32_t b = cs_div(row, a.by_K), k = row - b * a.c.K;
   const int W = a.c.W, keep = a.keep;
   const int32_t V = (int32_t)a.c.V;
-  float* out_x = a.item_x + (int64_t)item * keep;
-  int32_t* out_v = a.item_v + (int64_t)item * keep;
   if (a.finished && a.finished[row]) {   // its one candidate keeps the beam's score; its logits are not read
     if (lane == 0) {
-      a.stat[item] = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
+      *stat = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
       if (base == 0) { out_x[0] = 0.0f; out_v[0] = (int32_t)a.c.end_token; }
     }
     return;
@@ -352,13 +348,22 @@ __global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
       n = n < W ? n : W;
     }
   }
-  if (lane == 0) a.stat[item] = BmStat{ref, sum, top, n};
+  if (lane == 0) *stat = BmStat{ref, sum, top, n};
+}
+
+template <typename T, bool MASK, int LANE>
+__global__ void __launch_bounds__(256) cs_beam_scan_kernel(const BmArgs a) {
+  const uint32_t item = cs_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (item >= a.items) return;
+  const uint32_t row = cs_div(item, a.by_stretches);
+  const int64_t at = (int64_t)item * a.keep;
+  bm_scan<T, MASK, LANE>(a, row, item - row * a.stretches, a.stat + item, a.item_x + at, a.item_v + at);
 }
 
 // One workgroup per example; bound by its chain of dependent loads and barriers: 5.9 us for 4 beams of 32 stretches, 16 for 16 of
-// 64, 12 for 4096 examples of 5 stretches.
-__global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, int cap) {
-  extern __shared__ char lds[];
+// 64, 10 for 4096 examples of 5 stretches (W = 64: 34).
+__device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat* stat, const float* item_x, const int32_t* item_v,
+                                        char* lds, int cap) {
   double* s_lse = (double*)lds;                                     // [K]
   double* s_before = s_lse + a.c.K;                                 // [K] scores
   uint64_t* s_key = (uint64_t*)(s_before + a.c.K);                  // [cap] scores of candidates, as ordered bits
@@ -369,13 +374,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   __shared__ int s_n, s_left;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, waves = threads >> 6;
-  const int64_t b = cs_block();
-  if (b >= a.c.B) return;
   const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
   const int32_t total = K * C;         // (at most 2^31 / keep, checked on the host)
-  const BmStat* stat = a.stat + b * total;
-  const float* item_x = a.item_x + b * total * keep;
-  const int32_t* item_v = a.item_v + b * total * keep;
   constexpr double INF = __builtin_inf();
   // (asked for before the normalisers are formed)
   const float top0 = tid < total ? stat[tid].top : -__builtin_inff();
@@ -383,16 +383,23 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   const int n_first = total <= 64 && lane < total ? stat[lane].n : 0;
   const BmPow pow(lane);
   if (tid == 0) { s_n = 0; s_left = 0; }
-  for (int k = wave; k < K; k += waves) {
-    const int64_t row = b * K + k;
+  // the lanes of a beam: a power of two
+  int g = 1;
+  while (g < C && g < 64) g *= 2;
+  const int per = 64 / g, sub = lane & (g - 1);
+  for (int k0 = wave * per; k0 < K; k0 += waves * per) {
+    const int k = k0 + lane / g;
+    const bool mine = k < K;
+    const int64_t row = b * K + (mine ? k : K - 1);
     double before = 0.0, lse = 0.0;
     if (a.scores) before = a.c.scores_type == CS_TYPE_F64 ? ((const double*)a.scores)[row] : (double)((const float*)a.scores)[row];
-    if (a.c.normalise && !(a.finished && a.finished[row])) {
+    const bool formed = mine && a.c.normalise && !(a.finished && a.finished[row]);
+    if (__ballot(formed)) {
       const BmStat* st = stat + k * C;
       // Lanes join their stretches, then each other: those of reference 0 (the rule) and, apart, the others.
       float top = -__builtin_inff();               // of the former
       double sum = 0.0, ref = -INF, far = 0.0;     // far: of the latter, relative to ref
-      for (int c = lane; c < C; c += 64) {
+      for (int c = sub; formed && c < C; c += g) {
         const BmStat s = st[c];
         if (s.sum != s.sum) sum = s.sum;             // (NaN stays)
         if (!(s.top > -__builtin_inff())) continue;  // nothing allowed there
@@ -405,28 +412,32 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
           ref = m;
         }
       }
-      top = bm_wave_max(top);
-      sum = bm_wave_sum(sum);
+      if (g == 64) {
+        top = bm_wave_max(top);
+        sum = bm_wave_sum(sum);
+      } else {
+        for (int o = g >> 1; o; o >>= 1) {
+          top = fmaxf(top, __shfl_xor(top, o));
+          sum += __shfl_xor(sum, o);
+        }
+      }
       double m = (double)top;
       if (__ballot(ref > -INF)) {
         double all = ref;
-        for (int o = 32; o; o >>= 1) all = fmax(all, __shfl_xor(all, o));
-        far = bm_wave_sum(ref > -INF ? far * exp(ref - all) : far);
-        ref = all;
-        m = fmax(m, ref);
-        far *= exp(ref - m);
+        for (int o = g >> 1; o; o >>= 1) all = fmax(all, __shfl_xor(all, o));
+        far = ref > -INF ? far * exp(ref - all) : far;
+        for (int o = g >> 1; o; o >>= 1) far += __shfl_xor(far, o);
+        m = fmax(m, all);
+        far = all > -INF ? far * exp(all - m) : far;
       }
       // The sum relative to the largest logit, that logit's own part being one exactly: a beam left with one value has a
       // normaliser of just its logit, and of a beam that is all but certain the rest counts, not the roundings of the whole.
-      if (m == (double)top && top > -__builtin_inff()) {
-        const double e = bm_add_exp(0.0, m, pow);
-        sum = 1.0 + (sum - e) / e;
-      } else if (top > -__builtin_inff()) {
-        sum *= exp(-m);
-      }
-      lse = m + log(sum + far);        // (+inf, NaN or nothing allowed: NaN or -inf, with no candidate left to count)
+      const double e = bm_add_exp(0.0, m, pow);      // (all lanes have to be there)
+      if (m == (double)top) sum = 1.0 + (sum - e) / e;
+      else if (top > -__builtin_inff()) sum *= exp(-m);
+      lse = formed ? m + log(sum + far) : 0.0;       // (+inf, NaN or nothing allowed: NaN or -inf, with no candidate left to count)
     }
-    if (lane == 0) { s_lse[k] = lse; s_before[k] = before; }
+    if (mine && sub == 0) { s_lse[k] = lse; s_before[k] = before; }
   }
   __syncthreads();
   auto key_of = [&](float x, int g) {   // (in this order: where x is the whole normaliser, the score stays what it was)
@@ -435,7 +446,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   };
   // a bound from below; none where there are few candidates
   uint64_t t = 1;
-  if (total > 64 || bm_wave_sum((double)n_first) > cap / 2) {
+  if (total > 64 || bm_wave_sum((double)n_first) > 2 * W + 64) {
     // the W-th largest score, as far as its leading 32 bits say, among the lanes' best of a wavefront: of the stretches' largest
     // logits or, where these are few, of all kept ones
     uint32_t best = 0;
@@ -519,10 +530,10 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   };
   const int n = s_n;
   if (n <= cap) {
-    // ranks by counting: each candidate against all.  Where there are many (W above 32), those from a bound on that W to 128
-    // more reach, bisected: 600 candidates against all took one wavefront 390 us
-    int left = n;
-    if (n > 2 * W + 128) {
+    // ranks by counting: each candidate against all.  Where there are many (W above 32), those from a bound on that W to 32
+    // more reach, bisected
+    int m = n;
+    if (n > W + 96) {
       uint64_t most = 0;
       for (int i = tid; i < n; i += threads) most = s_key[i] > most ? s_key[i] : most;
       for (int o = 32; o; o >>= 1) {
@@ -534,7 +545,8 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
       __syncthreads();
       for (int w = 0; w < waves; ++w) most = s_wave[w] > most ? s_wave[w] : most;
       uint64_t lo = t, hi = most + 1;              // W or more reach lo, none hi
-      while (left > W + 128 && hi - lo > 1) {
+      int left = n;
+      while (left > W + 32 && hi - lo > 1) {
         const uint64_t mid = lo + (hi - lo) / 2;
         __syncthreads();
         if (tid == 0) s_left = 0;
@@ -547,29 +559,38 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
         if (s_left < W) hi = mid;
         else { lo = mid; left = s_left; }
       }
-      __syncthreads();
-      if (tid == 0) s_left = 0;
-      __syncthreads();
-      if (left <= W + 128)                         // (else that many are equal: all stay)
+      if (left <= W + 32) {                        // (else that many are equal: all stay)
+        __syncthreads();
+        if (tid == 0) s_left = 0;
+        __syncthreads();
         for (int i = tid; i < n; i += threads)
           if (s_key[i] >= lo) s_open[atomicAdd(&s_left, 1)] = i;
-      __syncthreads();
-    }
-    auto rank = [&](int m, auto place) {
-      for (int i = tid; i < m; i += threads) {
-        const uint64_t key = s_key[place(i)];
-        const int64_t at = s_at[place(i)];
-        int before = 0;
-#pragma unroll 4
-        for (int j = 0; j < m; ++j) {
-          const uint64_t other = s_key[place(j)];
-          before += other > key || (other == key && s_at[place(j)] < at);
-        }
-        if (before < W) put(before, key, at);
+        __syncthreads();
+        // they move to the front: two at most of a thread
+        const int i0 = tid < left ? s_open[tid] : 0, i1 = tid + 64 < left && tid < 64 ? s_open[tid + 64] : 0;
+        const uint64_t k0 = s_key[i0], k1 = s_key[i1];
+        const int64_t at0 = s_at[i0], at1 = s_at[i1];
+        __syncthreads();
+        if (tid < left && tid < 64) { s_key[tid] = k0; s_at[tid] = at0; }
+        if (tid + 64 < left && tid < 64) { s_key[tid + 64] = k1; s_at[tid + 64] = at1; }
+        __syncthreads();
+        m = left;
       }
-    };
-    if (left < n && left <= W + 128) rank(left, [&](int i) { return s_open[i]; });
-    else rank(n, [](int i) { return i; });
+    }
+    for (int i = tid; i < m; i += threads) {
+      const uint64_t key = s_key[i];
+      const int64_t at = s_at[i];
+      int before = 0, equal = 0;
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) {
+        const uint64_t other = s_key[j];
+        before += other > key;
+        equal += other == key;
+      }
+      if (equal > 1 && before < W)
+        for (int j = 0; j < m; ++j) before += s_key[j] == key && s_at[j] < at;
+      if (before < W) put(before, key, at);
+    }
     for (int w = n + tid; w < W; w += threads) put(w, 0, 0);
     return;
   }
@@ -603,10 +624,36 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   }
 }
 
-// values per lane of a stretch: 32 where that fills the chip (6 wavefronts on each of its 1024 SIMDs), else 16 or 8
+__global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, int cap) {
+  extern __shared__ __align__(16) char lds[];
+  const int64_t b = cs_block(), total = (int64_t)a.c.K * a.stretches;
+  if (b >= a.c.B) return;
+  bm_join(a, b, a.stat + b * total, a.item_x + b * total * a.keep, a.item_v + b * total * a.keep, lds, cap);
+}
+
+// Both in one launch, where an example has few stretches: a wavefront each, which leave what they keep in LDS.  Saves a launch (512 x
+// 4 x 10: 12 us per call, not 15) and the way through memory (16384 x 4 x 2048: 132, not 165).  Where several stretches of 2048 make
+// a beam it loses, since a workgroup loads nothing while it joins (4096 x 10200: 67, not 47): there the two launches stay.
+template <typename T, bool MASK, int LANE>
+__global__ void __launch_bounds__(BM_ONE * 64) cs_beam_one_kernel(const BmArgs a, int cap) {
+  extern __shared__ __align__(16) char lds[];
+  const int64_t b = cs_block();
+  if (b >= a.c.B) return;
+  const int total = a.c.K * a.stretches, keep = a.keep;
+  BmStat* stat = (BmStat*)lds;
+  float* item_x = (float*)(stat + total);
+  int32_t* item_v = (int32_t*)(item_x + total * keep);
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = cs_div(w, a.by_stretches);
+  bm_scan<T, MASK, LANE>(a, (uint32_t)b * a.c.K + k, w - k * a.stretches, stat + w, item_x + w * keep, item_v + w * keep);
+  __syncthreads();
+  bm_join(a, b, stat, item_x, item_v, lds + total * (sizeof(BmStat) + keep * 8), cap);
+}
+
+// values per lane of a stretch: 32 where that fills the chip (6 wavefronts on each of its 1024 SIMDs), else, or where fewer hold
+// all values, 16 or 8
 int lane_values(const cs_beam_cfg& c) {
   int lane = 32;
-  while (lane > 8 && (int64_t)c.B * c.K * ((c.V + 64 * lane - 1) / (64 * lane)) < 6144) lane /= 2;
+  while (lane > 8 && (c.V <= 32 * lane || (int64_t)c.B * c.K * ((c.V + 64 * lane - 1) / (64 * lane)) < 6144)) lane /= 2;
   return lane;
 }
 int32_t stretches_of(const cs_beam_cfg& c) {
@@ -617,13 +664,19 @@ int32_t stretches_of(const cs_beam_cfg& c) {
 // W <= 32; for more, nearly all lanes count, their best tell little, and a better bound is bisected
 int32_t keep_of(const cs_beam_cfg& c) { return c.W <= 32 ? 2 * c.W + 32 : 96; }
 
+// the scan alone or, given its threads, the kernel that joins as well
+template <typename T, bool MASK, int LANE>
+void launch_stretches(const BmArgs& a, int threads, int lds, int cap, hipStream_t st) {
+  if (threads) hipLaunchKernelGGL((cs_beam_one_kernel<T, MASK, LANE>), cs_grid(a.c.B), dim3(threads), lds, st, a, cap);
+  else hipLaunchKernelGGL((cs_beam_scan_kernel<T, MASK, LANE>), cs_grid(((int64_t)a.items + 3) / 4), dim3(256), 0, st, a);
+}
 template <typename T>
-void launch_scan(const BmArgs& a, dim3 grid, hipStream_t st) {
+void launch_scan(const BmArgs& a, int threads, int lds, int cap, hipStream_t st) {
   switch (lane_values(a.c)) {
-#define CS_SCAN(L_)                                                                                              \
-    case L_:                                                                                                     \
-      if (a.mask) hipLaunchKernelGGL((cs_beam_scan_kernel<T, true, L_>), grid, dim3(256), 0, st, a);             \
-      else hipLaunchKernelGGL((cs_beam_scan_kernel<T, false, L_>), grid, dim3(256), 0, st, a);                   \
+#define CS_SCAN(L_)                                                                \
+    case L_:                                                                       \
+      if (a.mask) launch_stretches<T, true, L_>(a, threads, lds, cap, st);         \
+      else launch_stretches<T, false, L_>(a, threads, lds, cap, st);               \
       break;
     CS_SCAN(8) CS_SCAN(16) CS_SCAN(32)
 #undef CS_SCAN
@@ -674,27 +727,38 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   a.by_stretches = cs_div_by(a.stretches);
   a.by_K = cs_div_by(c->K);
   a.by_keep = cs_div_by(a.keep);
-  const dim3 grid = cs_grid((items + 3) / 4);
-  if (c->logits_type == CS_TYPE_F32) launch_scan<float>(a, grid, st);
-  else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, grid, st);
-  else launch_scan<_Float16>(a, grid, st);
-  CS_HIP(hipGetLastError());
-  // a wavefront per beam and a thread per stretch, as far as that goes
   const int64_t total = (int64_t)c->K * a.stretches;
-  int64_t waves = (total + 63) / 64;
-  waves = waves > c->K ? waves : c->K;
+  const bool one = total <= BM_ONE && (a.stretches == 1 || lane_values(*c) < 32);
+  // a thread per stretch, those of a beam in one wavefront, as far as that goes
+  int lanes = 1;
+  while (lanes < a.stretches && lanes < 64) lanes *= 2;
+  int64_t waves = ((total > c->K * lanes ? total : c->K * lanes) + 63) / 64;
+  // (16 lanes go through what is kept of a stretch: up to 4 wavefronts while the chip has room for them.  1024 x 4 x 8000, 16
+  // stretches: 36 us with 4, 45 with 1; 4096 x 1 x 32000, 16 as well: 122 with 4, 111 with 1)
+  int64_t few = total / 4 < 4 ? total / 4 : 4;
+  few = few < 4096 / c->B ? few : 4096 / c->B;
+  waves = few > waves ? few : waves;
   // (and for wide searches a thread for every 8 of some W candidates per stretch, so that the W-th largest of the threads' best
   // is a good bound)
   const int64_t wide = (total * c->W + 511) / 512;
   waves = c->W > 32 && wide > waves ? wide : waves;
-  const int threads = 64 * (int)(waves < BM_JOIN / 64 ? waves : BM_JOIN / 64);
+  waves = one ? total : waves < BM_JOIN / 64 ? waves : BM_JOIN / 64;
+  const int threads = 64 * (int)waves;
   // places for what reaches the joined bound
   const int least = threads == 64 ? 128 : 1024, most = c->K > 1024 ? 1024 : 2048;   // (64 KB of LDS in all)
   int cap = c->W * 32;
   cap = cap > most ? most : cap < least ? least : cap;
-  hipLaunchKernelGGL(cs_beam_join_kernel, cs_grid(c->B), dim3(threads),
-                     (size_t)(c->K * 16 + cap * 16 + (threads < 192 ? 192 : threads) * 4), st, a, cap);
+  if (total <= 64 && cap > total * a.keep) cap = (int)total * a.keep;
+  const int lds = c->K * 16 + cap * 16 + (threads < 192 ? 192 : threads) * 4;
+  const int lds_one = lds + (int)total * (int)(sizeof(BmStat) + a.keep * 8);
+  if (c->logits_type == CS_TYPE_F32) launch_scan<float>(a, one ? threads : 0, lds_one, cap, st);
+  else if (c->logits_type == CS_TYPE_BF16) launch_scan<BmBf16>(a, one ? threads : 0, lds_one, cap, st);
+  else launch_scan<_Float16>(a, one ? threads : 0, lds_one, cap, st);
   CS_HIP(hipGetLastError());
+  if (!one) {
+    hipLaunchKernelGGL(cs_beam_join_kernel, cs_grid(c->B), dim3(threads), (size_t)lds, st, a, cap);
+    CS_HIP(hipGetLastError());
+  }
   return CS_OK;
 }
 
