@@ -386,3 +386,45 @@ def test_few_stretches_and_many_examples(B, K, V, W, kind):
         logits[1::3, :, V // 2:] -= 900
         logits[2::3, -1, : V // 3] = float("-inf")
     check(beam_select(scores, logits, W, **kw), scores, logits, W, **kw)
+
+
+@pytest.mark.parametrize("K", [1, 2, 4, 5, 8, 9, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("dtype,inner,skew", [(torch.uint8, 409, 1), (torch.uint8, 16, 3), (torch.uint8, 17, 0), (torch.uint8, 15, 0),
+                                              (torch.int16, 205, 1), (torch.int16, 8, 1), (torch.float32, 129, 1), (torch.float32, 64, 1),
+                                              (torch.float32, 63, 1), (torch.float32, 66, 2), (torch.float64, 33, 1),
+                                              (torch.float64, 34, 0)])
+def test_rows_of_every_length_and_alignment(dtype, inner, skew, K):
+    """Rows inside wider ones: what lies before and behind them stays."""
+    outer, B, pad = 3, 37, skew + 4
+    g = torch.Generator().manual_seed(inner + K)
+    wide = torch.randint(0, 200, (outer, B, K, inner + pad), generator=g).to(dtype).cuda()
+    parents = torch.arange(K).expand(B, K).clone()
+    for b in range(B):                                   # from none to all of the chains move, some of them nowhere
+        n = b % (K + 1)
+        parents[b, torch.randperm(K, generator=g)[:n]] = torch.randint(-1, K + 1, (n,), generator=g)
+    fine = (parents >= 0) & (parents < K)
+    at = torch.where(fine, parents, torch.arange(K)).cuda()
+    want = wide.clone()
+    rows = wide[..., skew:skew + inner]
+    want[..., skew:skew + inner] = torch.gather(rows, 2, at[None, :, :, None].expand(outer, B, K, inner))
+    held = wide.clone()
+    target = torch.zeros_like(wide)
+    reorder_states(rows, parents.cuda(), batch_dim=1, out=target[..., skew:skew + inner])
+    assert torch.equal(target[..., skew:skew + inner], torch.where(fine.cuda()[None, :, :, None], want[..., skew:skew + inner], 0))
+    assert not target[..., :skew].any() and not target[..., skew + inner:].any()
+    assert torch.equal(wide, held)
+    reorder_states(rows, parents.cuda(), batch_dim=1, out=rows)
+    assert torch.equal(wide, want)
+
+
+def test_more_than_four_billion_pieces_of_rows():
+    B = 290_000_000
+    rows = torch.empty(B, 2, 15, dtype=torch.uint8, device="cuda")
+    tag = torch.arange(2 * B, device="cuda").remainder_(251).to(torch.uint8).reshape(B, 2, 1)
+    rows.copy_(tag.expand_as(rows))
+    swap = torch.tensor([1, 0], device="cuda").expand(B, 2)
+    moved = reorder_states(rows, swap)
+    assert bool((moved == tag.flip(1)).all())
+    del moved
+    reorder_states(rows, swap, out=rows)
+    assert bool((rows == tag.flip(1)).all())

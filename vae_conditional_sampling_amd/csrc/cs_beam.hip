@@ -11,6 +11,7 @@
 // those of the definition.
 #include "cs_common.h"
 #include "cs_div.h"
+#include <type_traits>
 
 namespace {
 
@@ -772,63 +773,161 @@ struct BmMoveArgs {
   const char* src;
   char* dst;
   const int64_t* parents;
-  int64_t outer, B, cols;              // cols: vectors of a row
+  int64_t outer, B, cols;              // cols: pieces of a row
+  int64_t full;                        // the first ones are of the wider type, at any address
   int64_t ss[3], ds[3];                // bytes between outer / example / chain
   int32_t K, W;
   int64_t outer_step;                  // a thread serves every outer_step-th outer index
+  int32_t small;                       // all pieces of an outer index are less than 2^32
+  CsDiv by_cols, by_W;
 };
 
-// out of place: a thread per vector of a destination row, over its outer indices
-template <typename VEC>
+__device__ __forceinline__ int64_t bm_over(const BmMoveArgs& a, int64_t n, const CsDiv& by, int64_t d) {
+  return a.small ? (int64_t)cs_div((uint32_t)n, by) : n / d;
+}
+template <typename V> __device__ __forceinline__ V bm_get(const char* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <typename V> __device__ __forceinline__ void bm_put(char* p, V v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
+template <typename V>
+__device__ __forceinline__ void bm_gather(const BmMoveArgs& a, const char* s, char* d) {
+  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step) bm_put(d + o * a.ds[0], bm_get<V>(s + o * a.ss[0]));
+}
+// out of place: a thread per piece of a destination row, over its outer indices
+template <typename FULL, typename VEC>
 __global__ void __launch_bounds__(256) cs_beam_gather_kernel(const BmMoveArgs a) {
   const int64_t i = (int64_t)cs_block() * 256 + threadIdx.x;
   if (i >= a.B * a.W * a.cols) return;
-  const int64_t bw = i / a.cols, col = i - bw * a.cols;
+  const int64_t bw = bm_over(a, i, a.by_cols, a.cols), col = i - bw * a.cols;
   const int64_t p = a.parents[bw];
   if (p < 0 || p >= a.K) return;
-  const int64_t b = bw / a.W, w = bw - b * a.W;
-  const char* s = a.src + b * a.ss[1] + p * a.ss[2] + col * sizeof(VEC);
-  char* d = a.dst + b * a.ds[1] + w * a.ds[2] + col * sizeof(VEC);
-  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step)
-    *(VEC*)(d + o * a.ds[0]) = *(const VEC*)(s + o * a.ss[0]);
+  const int64_t b = bm_over(a, bw, a.by_W, a.W), w = bw - b * a.W;
+  const char* s = a.src + b * a.ss[1] + p * a.ss[2];
+  char* d = a.dst + b * a.ds[1] + w * a.ds[2];
+  if (sizeof(FULL) == sizeof(VEC) || col < a.full) {
+    bm_gather<FULL>(a, s + col * sizeof(FULL), d + col * sizeof(FULL));
+  } else {
+    const int64_t at = a.full * sizeof(FULL) + (col - a.full) * sizeof(VEC);
+    bm_gather<VEC>(a, s + at, d + at);
+  }
 }
 
-// in place: a thread owns one vector column of all K rows of an example, so it reads every row it needs before it
-// writes any; rows that keep their place are neither read nor written.  Bound by memory in whole lines of 128 bytes: half of
+// In place a thread owns one piece of all K rows of an example, so it reads every row it needs before it writes any; rows that
+// keep their place are neither read nor written.
+template <typename V, int KMAX>
+__device__ __forceinline__ void bm_move_few(const BmMoveArgs& a, char* d, const int (&parent)[KMAX]) {
+  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step) {
+    V v[KMAX];
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k)
+      if (parent[k] >= 0) v[k] = bm_get<V>(d + o * a.ds[0] + parent[k] * a.ds[2]);
+#pragma unroll
+    for (int k = 0; k < KMAX; ++k)
+      if (parent[k] >= 0) bm_put(d + o * a.ds[0] + k * a.ds[2], v[k]);
+  }
+}
+template <typename V, int KMAX, typename MASK>
+__device__ __forceinline__ void bm_move(const BmMoveArgs& a, char* d, MASK moved, const uint8_t* parent) {
+  auto first = [](MASK m) { return sizeof(MASK) == 8 ? __builtin_ctzll(m) : __builtin_ctz((uint32_t)m); };
+  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step) {
+    char* at = d + o * a.ds[0];
+    V v[KMAX];
+    MASK rest = moved;
+#pragma unroll
+    for (int j = 0; j < KMAX; ++j)
+      if (rest) {
+        v[j] = bm_get<V>(at + parent[first(rest)] * a.ds[2]);
+        rest &= rest - 1;
+      }
+    rest = moved;
+#pragma unroll
+    for (int j = 0; j < KMAX; ++j)
+      if (rest) {
+        bm_put(at + first(rest) * a.ds[2], v[j]);
+        rest &= rest - 1;
+      }
+  }
+}
+
+// Up to 4 chains: each thread reads its example's parents.  Bound by memory in whole lines of 128 bytes: half of
 // 4 chains moved, 211 MB of moved bytes read and written, takes 50 us in rows of 128 bytes (4.2 TB/s), 44 in rows of 1 KB and
 // 80 in rows of 172 bytes, whose ends share lines with rows that stay.  (There, 16 bytes a lane measured 81, scalar parents
 // with several columns a lane 86, streaming stores and loads 93 and 107.)
-template <typename VEC, int KMAX>
-__global__ void __launch_bounds__(256) cs_beam_inplace_kernel(const BmMoveArgs a) {
+template <typename FULL, typename VEC>
+__global__ void __launch_bounds__(256) cs_beam_inplace_few_kernel(const BmMoveArgs a) {
   const int64_t i = (int64_t)cs_block() * 256 + threadIdx.x;
   if (i >= a.B * a.cols) return;
-  const int64_t b = i / a.cols, col = i - b * a.cols;
-  int parent[KMAX];
+  const int64_t b = bm_over(a, i, a.by_cols, a.cols), col = i - b * a.cols;
+  int parent[4];
 #pragma unroll
-  for (int k = 0; k < KMAX; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const int64_t p = k < a.K ? a.parents[b * a.K + k] : -1;
     parent[k] = p < 0 || p >= a.K || p == k ? -1 : (int)p;
   }
-  char* d = a.dst + b * a.ds[1] + col * sizeof(VEC);
-  for (int64_t o = blockIdx.z; o < a.outer; o += a.outer_step) {
-    VEC v[KMAX];
-#pragma unroll
-    for (int k = 0; k < KMAX; ++k)
-      if (parent[k] >= 0) v[k] = *(const VEC*)(d + o * a.ds[0] + parent[k] * a.ds[2]);
-#pragma unroll
-    for (int k = 0; k < KMAX; ++k)
-      if (parent[k] >= 0) *(VEC*)(d + o * a.ds[0] + k * a.ds[2]) = v[k];
-  }
+  char* d = a.dst + b * a.ds[1];
+  if (sizeof(FULL) == sizeof(VEC) || col < a.full) bm_move_few<FULL>(a, d + col * sizeof(FULL), parent);
+  else bm_move_few<VEC>(a, d + a.full * sizeof(FULL) + (col - a.full) * sizeof(VEC), parent);
 }
 
-template <typename VEC>
-void launch_move(const BmMoveArgs& a, bool in_place, dim3 grid, hipStream_t st) {
-  if (!in_place) hipLaunchKernelGGL(cs_beam_gather_kernel<VEC>, grid, dim3(256), 0, st, a);
-  else if (a.K <= 4) hipLaunchKernelGGL((cs_beam_inplace_kernel<VEC, 4>), grid, dim3(256), 0, st, a);
-  else if (a.K <= 8) hipLaunchKernelGGL((cs_beam_inplace_kernel<VEC, 8>), grid, dim3(256), 0, st, a);
-  else if (a.K <= 16) hipLaunchKernelGGL((cs_beam_inplace_kernel<VEC, 16>), grid, dim3(256), 0, st, a);
-  else if (a.K <= 32) hipLaunchKernelGGL((cs_beam_inplace_kernel<VEC, 32>), grid, dim3(256), 0, st, a);
-  else if constexpr (sizeof(VEC) <= 8) hipLaunchKernelGGL((cs_beam_inplace_kernel<VEC, 64>), grid, dim3(256), 0, st, a);
+// More: the workgroup's parents lie in LDS and a thread goes through the bits of the rows that move alone (2 of 10 rows of 818 bytes:
+// 11 us; with a test per chain and the parents in registers 23).
+template <typename FULL, typename VEC, int KMAX>
+__global__ void __launch_bounds__(256) cs_beam_inplace_kernel(const BmMoveArgs a) {
+  using MASK = typename std::conditional<(KMAX > 32), unsigned long long, unsigned>::type;
+  constexpr int EXAMPLES = 257;        // of a workgroup, at most
+  __shared__ MASK s_moved[EXAMPLES];
+  __shared__ uint8_t s_parent[EXAMPLES * KMAX];
+  const int tid = threadIdx.x;
+  const int64_t pieces = a.B * a.cols, i0 = (int64_t)cs_block() * 256;
+  if (i0 >= pieces) return;
+  const int64_t i = i0 + tid < pieces ? i0 + tid : pieces - 1, last = i0 + 255 < pieces ? i0 + 255 : pieces - 1;
+  const int64_t b0 = bm_over(a, i0, a.by_cols, a.cols), b = bm_over(a, i, a.by_cols, a.cols);
+  const int examples = (int)(bm_over(a, last, a.by_cols, a.cols) - b0) + 1;
+  for (int e = tid; e < examples; e += 256) s_moved[e] = 0;
+  __syncthreads();
+  for (int e = tid; e < examples * a.K; e += 256) {
+    const int x = (int)cs_div((uint32_t)e, a.by_W), k = e - x * a.K;     // (W = K)
+    const int64_t p = a.parents[b0 * a.K + e];
+    if (p >= 0 && p < a.K && p != k) {
+      s_parent[x * KMAX + k] = (uint8_t)p;
+      atomicOr(&s_moved[x], (MASK)1 << k);
+    }
+  }
+  __syncthreads();
+  if (i0 + tid >= pieces) return;
+  const MASK moved = s_moved[b - b0];
+  const uint8_t* parent = s_parent + (b - b0) * KMAX;
+  const int64_t col = i - b * a.cols;
+  char* d = a.dst + b * a.ds[1];
+  if (sizeof(FULL) == sizeof(VEC) || col < a.full) bm_move<FULL, KMAX>(a, d + col * sizeof(FULL), moved, parent);
+  else bm_move<VEC, KMAX>(a, d + a.full * sizeof(FULL) + (col - a.full) * sizeof(VEC), moved, parent);
+}
+
+// The bytes of a piece where starts and ends of all rows are multiples of `unit` bytes: the unit, or 16 (8, 4 where a thread holds more
+// than 16, 32 of them) at any address and what is left of a row in units.  The latter pays where a row has many units: 785 bytes in 5
+// chains, 2 moved: 81 us, not 191; 1700 bytes, out of place: 44, not 57; but 172 bytes: 34, not 30.
+int piece_of(int unit, int64_t row_bytes, bool in_place, int K) {
+  const int widest = !in_place || K <= 16 ? 16 : K <= 32 ? 8 : 4;
+  return unit <= 2 || (unit == 4 && row_bytes >= 256) || unit > widest ? widest : unit;
+}
+template <typename FULL, typename VEC>
+void launch_pieces(const BmMoveArgs& a, bool in_place, dim3 grid, hipStream_t st) {
+  if (!in_place) hipLaunchKernelGGL((cs_beam_gather_kernel<FULL, VEC>), grid, dim3(256), 0, st, a);
+  else if (a.K <= 4) hipLaunchKernelGGL((cs_beam_inplace_few_kernel<FULL, VEC>), grid, dim3(256), 0, st, a);
+  else if (a.K <= 8) hipLaunchKernelGGL((cs_beam_inplace_kernel<FULL, VEC, 8>), grid, dim3(256), 0, st, a);
+  else if (a.K <= 16) hipLaunchKernelGGL((cs_beam_inplace_kernel<FULL, VEC, 16>), grid, dim3(256), 0, st, a);
+  else if constexpr (sizeof(FULL) == 8) hipLaunchKernelGGL((cs_beam_inplace_kernel<FULL, VEC, 32>), grid, dim3(256), 0, st, a);
+  else if constexpr (sizeof(FULL) == 4) hipLaunchKernelGGL((cs_beam_inplace_kernel<FULL, VEC, 64>), grid, dim3(256), 0, st, a);
+}
+template <typename FULL>
+void launch_units(const BmMoveArgs& a, int unit, bool in_place, dim3 grid, hipStream_t st) {
+  if (unit == (int)sizeof(FULL)) launch_pieces<FULL, FULL>(a, in_place, grid, st);
+  else if (unit == 2) launch_pieces<FULL, uint16_t>(a, in_place, grid, st);
+  else if (unit == 1) launch_pieces<FULL, uint8_t>(a, in_place, grid, st);
+  else if constexpr (sizeof(FULL) > 4) launch_pieces<FULL, uint32_t>(a, in_place, grid, st);
 }
 
 }  // namespace
@@ -871,10 +970,17 @@ extern "C" int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_
     if (n_src[i] > 1) bits |= (uintptr_t)src_stride[i];
     if (n_dst[i] > 1) bits |= (uintptr_t)dst_stride[i];
   }
-  // (64 rows of 16-byte columns would not fit a thread's registers)
-  const int vec = (bits & 15) == 0 && !(in_place && K > 32) ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
-  a.cols = row_bytes / vec;
-  const int64_t blocks = (B * (in_place ? 1 : W) * a.cols + 255) / 256;
+  int unit = 1;
+  while (unit < 16 && (bits & unit) == 0) unit *= 2;
+  const int piece = piece_of(unit, row_bytes, in_place, K);
+  unit = unit < piece ? unit : piece;
+  a.full = row_bytes / piece;
+  a.cols = a.full + (row_bytes - a.full * piece) / unit;
+  const int64_t rows = B * (in_place ? 1 : W);
+  a.small = rows * a.cols <= UINT32_MAX;
+  a.by_cols = cs_div_by(a.small ? a.cols : 1);
+  a.by_W = cs_div_by(W);
+  const int64_t blocks = (rows * a.cols + 255) / 256;
   CS_REQUIRE(blocks <= INT32_MAX, "too many states for one call");
   // a thread serves several outer indices once that still leaves the chip full
   int64_t split = (8192 + blocks - 1) / blocks;
@@ -884,11 +990,9 @@ extern "C" int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_
   dim3 grid = cs_grid(blocks);
   grid.z = (unsigned)a.outer_step;
   hipStream_t st = (hipStream_t)stream;
-  if (vec == 16) launch_move<u32x4>(a, in_place, grid, st);
-  else if (vec == 8) launch_move<u32x2>(a, in_place, grid, st);
-  else if (vec == 4) launch_move<uint32_t>(a, in_place, grid, st);
-  else if (vec == 2) launch_move<uint16_t>(a, in_place, grid, st);
-  else launch_move<uint8_t>(a, in_place, grid, st);
+  if (piece == 16) launch_units<u32x4>(a, unit, in_place, grid, st);
+  else if (piece == 8) launch_units<u32x2>(a, unit, in_place, grid, st);
+  else launch_units<uint32_t>(a, unit, in_place, grid, st);
   CS_HIP(hipGetLastError());
   return CS_OK;
 }
