@@ -164,8 +164,8 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
   return t;
 }
 
-// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 654 of them for 2048 values, 364 of
-// these the 64-bit exponentials (91 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 85 to 92 us, 85 % of
+// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 618 of them for 2048 values, 364 of
+// these the 64-bit exponentials (91 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 82 to 90 us, 85 % of
 // them issuing, where their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
 // (Logits and values kept in two arrays, so that a kept one costs 4 instructions and not 8: 3 % faster.)
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the

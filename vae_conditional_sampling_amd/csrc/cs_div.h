@@ -5,17 +5,17 @@
 #include <stdint.h>
 
 struct CsDiv {
-  uint32_t d, mul, shift;
+  uint32_t d, mul, s1, s2;
 };
 inline CsDiv cs_div_by(int64_t d) {
   uint32_t l = 0;
   while (l < 32 && (1ull << l) < (uint64_t)d) ++l;
   const uint64_t mul = ((1ull << 32) * ((1ull << l) - (uint64_t)d)) / (uint64_t)d + 1;
-  return CsDiv{(uint32_t)d, (uint32_t)mul, l};
+  return CsDiv{(uint32_t)d, (uint32_t)mul, l ? 1u : 0u, l ? l - 1 : 0u};
 }
-__device__ __forceinline__ uint32_t cs_div(uint32_t n, const CsDiv& d) {
+__device__ __forceinline__ uint32_t cs_div(uint32_t n, const CsDiv& d) {   // (scalar instructions where n is uniform)
   const uint32_t t = __umulhi(n, d.mul);
-  return d.shift == 0 ? n : (t + ((n - t) >> 1)) >> (d.shift - 1);
+  return (t + ((n - t) >> d.s1)) >> d.s2;
 }
 
 // Workgroups of 256 to 1024 threads in two axes (an axis of a launch has to stay below 2^32 threads), and the number of one;
