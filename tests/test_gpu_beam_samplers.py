@@ -131,3 +131,28 @@ def test_both_options_through_the_yaml_driver(tmp_path):
     m = np.broadcast_to(f["masks"][None], f["imputations"].shape)
     assert np.isfinite(f["imputations"]).all()
     assert np.array_equal(f["imputations"][m], np.broadcast_to(f["true_X"][None], m.shape)[m])
+
+
+def test_binary_data_keep_their_uint8_history():
+    from tests.helpers import conv_weights, make_conv_model
+    from tests.test_gpu_samplers import BASE_KW
+    from vae_conditional_sampling_amd.sampling import test_step_vae_sampling as T
+    enc_w, dec_w = conv_weights("omni_like", 7)
+    g = torch.Generator().manual_seed(5)
+    B, K, D = 3, 4, 784
+    X0 = (torch.rand(B, 1, D, generator=g) < 0.3).float().repeat(1, K, 1)
+    M = torch.rand(B, 1, D, generator=g) < 0.5
+    runs = []
+    for fmt in (None, "int8"):
+        s = T.TestVAELatentAdaptiveImportanceResampling(
+            num_iterations=6, num_imp_samples=1, weighting_scheme="dmis", resampling_scheme="gr", resampling_method="multinomial",
+            num_prior_replenish_proposals=1, num_pseudo_warmup_iterations=1, num_historical_proposals=2,
+            no_historic_proposals_iterations=3, imputation_history_length=4, imputation_history_format=fmt, num_copies=K, **BASE_KW)
+        s.set_model(make_conv_model("omni_like", enc_w, dec_w, "normal", "bern"))
+        s.on_test_start()
+        s.rng_seed = 11
+        s.on_test_batch_start(None, 0)
+        Xi = s.basic_imputation(X0.cuda(), M.cuda())
+        runs.append([d["X"].clone() for d in s.sampler(Xi, M.cuda())])
+    assert len(runs[0]) == len(runs[1]) and all(torch.equal(a, b) for a, b in zip(*runs))
+    assert not torch.equal(runs[0][0], runs[0][-1])

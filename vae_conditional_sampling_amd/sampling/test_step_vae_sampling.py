@@ -599,9 +599,10 @@ class TestVAELatentAdaptiveImportanceResampling(TestVAESamplerBase):
         B, K, D = X.shape
         history = None
         if hp.num_historical_proposals is not None:   # :1866-1870
+            binary = _check_if_bool(X)                # (its history has 8 bits as it is)
             history = ImputationHistoryQueue(max_history_length=hp.imputation_history_length, batch_shape=X.shape,
-                                             dtype=torch.bool if _check_if_bool(X) else torch.float32, device=X.device,
-                                             storage=hp.imputation_history_format)
+                                             dtype=torch.bool if binary else torch.float32, device=X.device,
+                                             storage=None if binary else hp.imputation_history_format)
         clip_min = clip_max = None
         if hp.clip_imputations:
             X_temp = X[:, 0].clone()

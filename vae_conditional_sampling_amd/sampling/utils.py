@@ -83,9 +83,9 @@ class ImputationHistoryQueue(object):
         Xc = out if out is not None else torch.empty(B, K + H, D, device=X.device, dtype=torch.float32)
         if self.quantised is not None:
             Xc[:, :K] = X
-            at = torch.tensor(slots, device=X.device).expand(B, H)
+            at = torch.tensor(slots, dtype=torch.int64, device=X.device).expand(B, H)
             if chain_of_proposal is not None:
-                chains = torch.tensor([int(c) for c in chain_of_proposal], device=X.device).expand(B, H)
+                chains = torch.tensor([int(c) for c in chain_of_proposal], dtype=torch.int64, device=X.device).expand(B, H)
             elif chain_of_example is not None:
                 chains = chain_of_example.to(X.device, torch.int64)[:, None].expand(B, H)
             else:
