@@ -22,8 +22,9 @@ struct QcArgs {
   cs_qcache c;
   int64_t record;              // bytes
   int32_t code_bytes;          // of a record, rounded up to 4
-  int32_t lanes;               // lanes of a row: groups * G / 8
+  int32_t lanes;               // lanes of a row: write: groups * G / 8; read: D / 8, rounded up
   int32_t rows_per_block;
+  int32_t lg_shift;            // 2^lg_shift lanes share a group's scale
   uint32_t rows;               // rows of the call, below 2^31
   CsDiv by_lanes, by_chains, by_inner, by_T;   // lanes; B * K (write) or B * J (read); K or J; T
   const void* x;               // write
@@ -44,7 +45,7 @@ __device__ __forceinline__ void qc_store(QcBf16* p, float v) {   // nearest, tie
   p->u = (uint16_t)(v != v ? 0x7fc0u : (u + 0x7fffu + ((u >> 16) & 1)) >> 16);
 }
 
-// The largest of the lanes of a group (lg = 4, 8 or 16 neighbouring lanes): exchanges within quads, then the mirrored other
+// The largest of the lanes of a group (lg = 1 to 16 neighbouring lanes): exchanges within quads, then the mirrored other
 // half of 8 and of 16 lanes, whose halves are of one value by then.
 __device__ __forceinline__ uint32_t qc_group_max(uint32_t v, int lg) {
 #define CS_STEP(CTRL_)                                                                                        \
@@ -52,7 +53,8 @@ __device__ __forceinline__ uint32_t qc_group_max(uint32_t v, int lg) {
     const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL_, 0xf, 0xf, false);         \
     v = o > v ? o : v;                                                                                        \
   }
-  CS_STEP(0xb1) CS_STEP(0x4e)            // quad_perm: 1 0 3 2, 2 3 0 1
+  if (lg > 1) CS_STEP(0xb1)              // quad_perm: 1 0 3 2
+  if (lg > 2) CS_STEP(0x4e)              // quad_perm: 2 3 0 1
   if (lg > 4) CS_STEP(0x141)             // row_half_mirror
   if (lg > 8) CS_STEP(0x140)             // row_mirror
 #undef CS_STEP
@@ -65,8 +67,12 @@ template <int FMT, bool PLAIN>
 __device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, uint32_t* codes, uint32_t* scale) {
   auto finite = [](float v) { return PLAIN || __builtin_fabsf(v) <= 3.402823466e+38f; };
   if (FMT == CS_QFMT_INT8) {
-    const float s = fmaxf(top / 127.0f, 1.17549435e-38f);
-    const float inv = 1.0f / s;
+    // top / 127 as division rounds it: one remainder corrects the product with fl(1/127) (Markstein 1990; below 127 * 2^-126, where
+    // remainders would not be exact, the scale does not depend on it)
+    constexpr float INV127 = 1.0f / 127.0f;
+    const float q127 = top * INV127;
+    const float s = fmaxf(__builtin_fmaf(__builtin_fmaf(-q127, 127.0f, top), INV127, q127), 1.17549435e-38f);
+    const float inv = __builtin_amdgcn_rcpf(s);   // (a unit in the last place off at most)
     float q[QC_LANE];
     bool near = false;
 #pragma unroll
@@ -76,7 +82,7 @@ __device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, 
       near = near || __builtin_fabsf(v - q[i]) > 0.4999f;
     }
     if (__ballot(near)) {
-      // v is off by less than 2e-5, so these alone can be beside the nearest integer of the real quotient: the remainder
+      // v is off by less than 3e-5, so these alone can be beside the nearest integer of the real quotient: the remainder
       // x - q s is exact (a multiple of the last place of s or x, below 2^24 of them) and says so
 #pragma unroll
       for (int i = 0; i < QC_LANE; ++i) {
@@ -196,7 +202,7 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
   const uint32_t b = cs_div(chain, a.by_inner), k = chain - b * a.by_inner.d;
   const T* x = (const T*)a.x + i * a.stride[0] + b * a.stride[1] + k * a.stride[2];
   char* rec = (char*)a.c.data + ((int64_t)slot * a.by_chains.d + chain) * a.record;
-  const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
+  const int D = a.c.D, lg = 1 << a.lg_shift;
   // (lanes of a row: a multiple of the lanes of a group, which divide 64)
   for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
     const int d0 = l * QC_LANE;
@@ -233,9 +239,9 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
     const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
     if (c0 < a.code_bytes) *(uint32_t*)(rec + c0) = codes[0];
     if (FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes) *(uint32_t*)(rec + c0 + 4) = codes[1];
-    if (l % lg == 0) {
-      if (FMT == CS_QFMT_INT8) *(uint32_t*)(rec + a.code_bytes + 4 * (l / lg)) = scale;
-      else *(uint8_t*)(rec + a.code_bytes + l / lg) = (uint8_t)scale;
+    if ((l & (lg - 1)) == 0) {
+      if (FMT == CS_QFMT_INT8) *(uint32_t*)(rec + a.code_bytes + 4 * (l >> a.lg_shift)) = scale;
+      else *(uint8_t*)(rec + a.code_bytes + (l >> a.lg_shift)) = (uint8_t)scale;
     }
   }
 }
@@ -270,7 +276,7 @@ __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
     out[r] = PACKED ? s_out + (r * a.rows_per_block + ry) * a.c.D
                     : (T*)a.out + i * a.stride[0] + b * a.stride[1] + j * a.stride[2];
   }
-  const int D = a.c.D, G = a.c.group, lg = G / QC_LANE;
+  const int D = a.c.D;
   for (int l = threadIdx.x - ry * a.lanes; l < a.lanes; l += 256) {
     const int d0 = l * QC_LANE;
     if (d0 >= D) break;
@@ -280,7 +286,8 @@ __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
       const int c0 = FMT == CS_QFMT_MXFP4 ? d0 / 2 : d0;
       codes[r][0] = *(const uint32_t*)(rec[r] + c0);
       codes[r][1] = FMT != CS_QFMT_MXFP4 && c0 + 4 < a.code_bytes ? *(const uint32_t*)(rec[r] + c0 + 4) : 0;
-      scale[r] = FMT == CS_QFMT_INT8 ? *(const uint32_t*)(rec[r] + a.code_bytes + 4 * (l / lg)) : *(const uint8_t*)(rec[r] + a.code_bytes + l / lg);
+      scale[r] = FMT == CS_QFMT_INT8 ? *(const uint32_t*)(rec[r] + a.code_bytes + 4 * (l >> a.lg_shift))
+                                    : *(const uint8_t*)(rec[r] + a.code_bytes + (l >> a.lg_shift));
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -363,7 +370,10 @@ int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStr
   CS_REQUIRE(((uintptr_t)c.data & 15) == 0, "the ring must be 16-byte aligned");
   a.record = cs_qcache_record_bytes(c.fmt, c.group, c.D);
   a.code_bytes = (int32_t)code_bytes_of(c.fmt, c.D);
-  a.lanes = (c.D + c.group - 1) / c.group * (c.group / QC_LANE);
+  if (WRITE)
+    while (a.c.group > QC_LANE && c.D <= a.c.group / 2) a.c.group /= 2;   // (a row of one group, cut to what it holds)
+  a.lanes = WRITE ? (c.D + a.c.group - 1) / a.c.group * (a.c.group / QC_LANE) : (c.D + QC_LANE - 1) / QC_LANE;
+  a.lg_shift = __builtin_ctz((unsigned)(a.c.group / QC_LANE));   // (groups are powers of two)
   a.by_lanes = cs_div_by(a.lanes);
   a.rows_per_block = a.lanes >= 256 ? 1 : 256 / a.lanes;
   const uint32_t blocks = (a.rows + a.rows_per_block - 1) / a.rows_per_block;
