@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(256) cs_qcache_write_kernel(const QcArgs a) {
 // PACKED: the rows of the call follow each other in `out` and their length is no multiple of 8 values.  Then the lanes' pieces
 // of a row would be stored in up to 8 parts each, every one of them touching all lines of the block's rows; the block's
 // rows are put together in LDS instead and stored as one run of 16-byte pieces: 524288 rows of 21 float32 from scattered records
-// in 21 us, 31 without (R = 4: 26).  Rows of more than 16 lanes gain nothing by it.
+// in 18.5 us, 30 without.  Rows of more than 16 lanes gain nothing by it.
 template <int FMT, typename T, int R, bool PACKED>
 __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
   extern __shared__ __align__(16) char lds[];
