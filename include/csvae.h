@@ -543,7 +543,8 @@ int cs_qcache_write(const cs_qcache* c, const void* X, int32_t x_type, int64_t n
                     const int64_t* start, int64_t start0, const int64_t* count, void* stream);
 /* out[i,b,j,:] = the state at slot slots[i,b,j] (NULL: (start0 + i) mod T) of chain chains[i,b,j] (NULL: j, and J must
  * be K) of example b; zeros where slot or chain do not exist.  slots / chains: int64 [N,B,J]; out_stride of
- * (i, example, j) in elements; rows of out must not overlap. */
+ * (i, example, j) in elements; rows of out must not overlap.  A value beyond the largest finite one of out_type reads as that
+ * one: a finite state never reads as an infinity. */
 int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t start0, const int64_t* chains, int64_t N, int32_t J,
                    void* out, int32_t out_type, const int64_t out_stride[3], void* stream);
 

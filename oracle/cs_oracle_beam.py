@@ -56,7 +56,8 @@ def _nearest(a, grid):
 
 
 def quantised(x, fmt, group):
-    """What states x [...,D] (float32 values) read back as from a QuantisedHistory, in float64."""
+    """What states x [...,D] (float32 values) read back as from a QuantisedHistory in float32, in float64.  Read in a type of a
+    smaller range they are cut to its largest value."""
     x = np.asarray(x, dtype=np.float64)
     D = x.shape[-1]
     out = np.empty_like(x)
@@ -68,7 +69,6 @@ def quantised(x, fmt, group):
         if fmt == "int8":
             scale = np.maximum((top.astype(np.float32) / np.float32(127)), np.float32(2.0 ** -126)).astype(np.float64)
             r = np.clip(np.rint(v / scale), -127, 127) * scale
-            r = np.clip(r, -float(np.finfo(np.float32).max), float(np.finfo(np.float32).max))
             r = np.where(fine, r, np.nan)
         else:
             grid = E4M3 if fmt == "mxfp8" else E2M1
@@ -78,5 +78,7 @@ def quantised(x, fmt, group):
             scale = np.ldexp(1.0, e)
             r = np.copysign(_nearest(np.abs(v) / scale, grid) * scale, v)
             r = np.where(fine, r, np.nan) if fmt == "mxfp8" else np.where(fine.all(axis=-1, keepdims=True), r, np.nan)
+        # what a code or a scale rounds up beyond the largest float32 is cut to it (NaN stays)
+        r = np.clip(r, -float(np.finfo(np.float32).max), float(np.finfo(np.float32).max))
         out[..., lo:lo + group] = r
     return out

@@ -38,6 +38,11 @@ struct QcBf16 { uint16_t u; };
 __device__ __forceinline__ float qc_float(float v) { return v; }
 __device__ __forceinline__ float qc_float(_Float16 v) { return (float)v; }
 __device__ __forceinline__ float qc_float(QcBf16 v) { return __uint_as_float((uint32_t)v.u << 16); }
+// The largest finite value of the type that is read: what rounds up beyond it (a code to the next power of two, the scale of the
+// very largest states) is cut to it, so that a finite state reads as a finite value.
+template <typename T> struct QcMost { static constexpr float value = 3.402823466e+38f; static constexpr int e = 127; };   // (2 - ulp) 2^e
+template <> struct QcMost<_Float16> { static constexpr float value = 65504.0f; static constexpr int e = 15; };
+template <> struct QcMost<QcBf16> { static constexpr float value = 3.389531389e+38f; static constexpr int e = 127; };
 __device__ __forceinline__ void qc_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void qc_store(_Float16* p, float v) { *p = (_Float16)v; }
 __device__ __forceinline__ void qc_store(QcBf16* p, float v) {   // nearest, ties to even
@@ -132,16 +137,16 @@ __device__ __forceinline__ void qc_encode(const float* x, float top, bool fine, 
   *scale = FMT == CS_QFMT_MXFP4 && !fine ? 255u : (uint32_t)(e + 127);
 }
 
-template <int FMT>
+template <int FMT, typename T>
 __device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale, float* v) {
+  constexpr float most = QcMost<T>::value;
   typedef float f2 __attribute__((ext_vector_type(2)));
   if (FMT == CS_QFMT_INT8) {
     const float s = __uint_as_float(scale);
 #pragma unroll
     for (int i = 0; i < QC_LANE; ++i) {
       const int q = (int8_t)(codes[i >> 2] >> (8 * (i & 3)));
-      // (the scale of the very largest float32 values is rounded up: their product is kept finite)
-      const float p = fminf(fmaxf((float)q * s, -3.402823466e+38f), 3.402823466e+38f);
+      const float p = fminf(fmaxf((float)q * s, -most), most);
       v[i] = q == -128 ? __builtin_nanf("") : p;
     }
     return;
@@ -158,8 +163,18 @@ __device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale,
              c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 3);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
   }
+  // elements end at 1.75 * 2^8 and 1.5 * 2^2: no scale up to this one leaves the range
+  constexpr int SAFE = QcMost<T>::e - (FMT == CS_QFMT_MXFP8 ? 8 : 2);
+  if (__ballot(e > SAFE)) {
 #pragma unroll
-  for (int i = 0; i < QC_LANE; ++i) v[i] = scale == 255u ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v[i], e);
+    for (int i = 0; i < QC_LANE; ++i) {   // (a NaN stays: fmax and fmin would pass it over)
+      const float p = __builtin_amdgcn_ldexpf(v[i], e);
+      v[i] = scale == 255u ? __builtin_nanf("") : __builtin_fabsf(p) > most ? __builtin_copysignf(most, p) : p;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < QC_LANE; ++i) v[i] = __builtin_amdgcn_ldexpf(v[i], e);
 }
 
 // the slot of step i of a chain of a call that runs from `start` on; -1: not in the call
@@ -292,7 +307,7 @@ __global__ void __launch_bounds__(256) cs_qcache_read_kernel(const QcArgs a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float v[QC_LANE];
-      qc_decode<FMT>(codes[r], scale[r], v);
+      qc_decode<FMT, T>(codes[r], scale[r], v);
 #pragma unroll
       for (int e = 0; e < QC_LANE; ++e) v[e] = there[r] ? v[e] : 0.0f;
       if (!live[r]) continue;

@@ -262,7 +262,8 @@ class QuantisedHistory:
     def read(self, slots, chains=None, *, dtype=torch.float32, out=None):
         """``out[n,b,j] = state at slots[n,b,j] of chain chains[n,b,j]`` (None: of chain j) of example b, zeros where slot or
         chain do not exist.  ``slots`` / ``chains`` int64 [N,B,J] or [B,J]; ``out`` [N,B,J,D] (or [B,J,D]): any strides with D
-        adjacent."""
+        adjacent.  A value beyond the range of the type that is read becomes the type's largest (a finite state never reads as an
+        infinity)."""
         B, K, D = self.batch_shape
         shape = tuple(slots.shape)
         if len(shape) not in (2, 3) or shape[-2] != B or slots.dtype != torch.int64 or (chains is None and shape[-1] != K):
