@@ -506,7 +506,8 @@ int64_t cs_beam_select_workspace(const cs_beam_cfg* cfg);
  *   end_token with its score unchanged, and its logits are not read.
  * NaN and -inf are no candidates; a beam whose normaliser is not finite (a NaN or +inf among its allowed logits) has
  * none.  out_scores[B,W], parents[B,W], tokens[B,W] (int64); where there are fewer than W candidates: -inf, the
- * slot's own index (at most K-1), -1.  Candidates of one beam that 64 bits do not tell apart keep their logits' order.
+ * slot's own index (at most K-1), -1.  Scores that 64 bits do not tell apart are equal, whatever their logits: they go to the
+ * lowest k*V + v like all equal ones.
  * Two launches; the result does not depend on anything but the arguments. */
 int cs_beam_select(const cs_beam_cfg* cfg, const void* scores, const void* logits, const uint8_t* mask,
                    const uint8_t* finished, void* out_scores, int64_t* parents, int64_t* tokens, void* workspace,

@@ -6,7 +6,8 @@
 // stretch of one beam in registers (LANE values per lane), leaves their sum of exponentials and those of them that can
 // be among its W best in the workspace; a workgroup per example then joins the stretches of every beam, turns the
 // kept logits into scores and takes the W best of them.  The normaliser joins before scores of different beams are
-// compared, so within a beam a stretch's candidates can be chosen by their logits alone.  Sums and scores are held in
+// compared, so within a beam a stretch's candidates can be chosen by their logits alone; where 64 bits give different logits
+// one score, what such a choice left out is looked for once more (bm_join).  Sums and scores are held in
 // 64 bits: two beams' candidates are often closer than float32 sums of 10^5 terms are exact, and the indices are to be
 // those of the definition.
 #include "cs_common.h"
@@ -21,8 +22,10 @@ constexpr int BM_JOIN = 1024;          // threads that join an example, at most
 constexpr int BM_ONE = 8;              // stretches of an example, at most, for one launch that does it all
 constexpr float BM_LOWEST = -3.402823466e+38f;
 
-// of a stretch: the sum of exp(x - ref), the largest logit, the number of kept ones
-struct BmStat { double ref, sum; float top; int32_t n; };
+// of a stretch: the sum of exp(x - ref), ref being the largest logit or 0; the largest logit; the bound that all kept ones reach and
+// no others do; the number of kept ones.  NaN in the place of the bound: some that equal the last kept one were not kept, and
+// the largest of the smaller ones stands behind it in the list.
+struct BmStat { double sum; float ref, top, cut; int32_t n; };
 
 struct BmArgs {
   cs_beam_cfg c;
@@ -33,10 +36,18 @@ struct BmArgs {
   int32_t* item_v;  // and their values
   void* out_scores;
   int64_t *parents, *tokens;
-  int32_t stretches, keep;
+  int32_t stretches, keep, len;   // values of a stretch
   uint32_t items;          // B*K*stretches
   CsDiv by_stretches, by_K, by_keep;
 };
+
+// The kernel's arguments, read anew: without this those that one part of a kernel alone needs are loaded at its start and kept, or
+// spilled, to there.
+__device__ __forceinline__ const BmArgs& bm_args() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();   // (they are the first ones)
+  asm volatile("" : "+s"(p));
+  return *(const BmArgs*)p;
+}
 
 __device__ __forceinline__ uint32_t bm_key(float v) {
   const uint32_t u = __float_as_uint(v);
@@ -181,7 +192,7 @@ __device__ __forceinline__ void bm_scan(const BmArgs& a, uint32_t row, uint32_t 
   const int32_t V = (int32_t)a.c.V;
   if (a.finished && a.finished[row]) {   // its one candidate keeps the beam's score; its logits are not read
     if (lane == 0) {
-      *stat = BmStat{0.0, 0.0, base == 0 ? 0.0f : -INF, base == 0 ? 1 : 0};
+      *stat = BmStat{0.0, 0.0f, base == 0 ? 0.0f : -INF, BM_LOWEST, base == 0 ? 1 : 0};
       if (base == 0) { out_x[0] = 0.0f; out_v[0] = (int32_t)a.c.end_token; }
     }
     return;
@@ -191,7 +202,8 @@ __device__ __forceinline__ void bm_scan(const BmArgs& a, uint32_t row, uint32_t 
   constexpr int VECS = LANE / N;
   float x[LANE];
   float best = -INF, least = INF;      // (a NaN is passed over)
-  double ref = 0.0, sum = 0.0, sum1 = 0.0;
+  float ref = 0.0f;
+  double sum = 0.0, sum1 = 0.0;
   const BmPow pow(lane);
   uint32_t raw[VECS][4];
   if (!MASK && base + 64 * LANE <= V) {
@@ -275,13 +287,13 @@ __device__ __forceinline__ void bm_scan(const BmArgs& a, uint32_t row, uint32_t 
 #pragma unroll
       for (int i = 0; i < LANE; ++i) nan = nan || x[i] != x[i];
       if (top > -INF) {
-        ref = (double)top;
+        ref = top;
         // (less than exp(-690) counts as that; of an infinite top every difference is NaN or -inf)
 #pragma unroll
         for (int i = 0; i < LANE; ++i) {
           float xi = x[i];
           asm("" : "+v"(xi));   // (else the conversions of both branches are made above them and kept: 64 more registers)
-          sum = bm_add_exp(sum, fmax((double)xi - ref, -690.0), pow);
+          sum = bm_add_exp(sum, fmax((double)xi - (double)ref, -690.0), pow);
           if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -356,9 +368,22 @@ __device__ __forceinline__ void bm_scan(const BmArgs& a, uint32_t row, uint32_t 
         n += __shfl(incl, 63);
       }
       n = n < W ? n : W;
+      float down = -INF;
+#pragma unroll
+      for (int i = 0; i < LANE; ++i) {
+        float xi = x[i];
+        asm("" : "+v"(xi));   // (else the comparisons above are kept for these, 32 pairs of registers)
+        down = fmaxf(down, xi < t ? xi : -INF);
+      }
+      down = bm_wave_max(down);
+      if (lane == 0) {
+        out_x[n] = down;
+        *stat = BmStat{sum, ref, top, __builtin_nanf(""), n};
+      }
+      return;
     }
   }
-  if (lane == 0) *stat = BmStat{ref, sum, top, n};
+  if (lane == 0) *stat = BmStat{sum, ref, top, t, n};
 }
 
 // (float32 without a mask fits 6 wavefronts on a SIMD when asked to, 2 % faster; masked kernels spill and lose a quarter)
@@ -373,8 +398,8 @@ __global__ void __launch_bounds__(256, LANE == 32 && !MASK && BmElem<T>::N == 4 
 
 // One workgroup per example; bound by its chain of dependent loads and barriers: 5.9 us for 4 beams of 32 stretches, 16 for 16 of
 // 64, 10 for 4096 examples of 5 stretches (W = 64: 34).
-__device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat* stat, const float* item_x, const int32_t* item_v,
-                                        char* lds, int cap) {
+__device__ __forceinline__ void bm_join(int64_t b, BmStat* stat, float* item_x, int32_t* item_v, char* lds, int cap) {
+  const BmArgs& a = bm_args();
   double* s_lse = (double*)lds;                                     // [K]
   double* s_before = s_lse + a.c.K;                                 // [K] scores
   uint64_t* s_key = (uint64_t*)(s_before + a.c.K);                  // [cap] scores of candidates, as ordered bits
@@ -382,7 +407,8 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
   __shared__ uint64_t s_wave[BM_JOIN / 64];
   __shared__ int64_t s_wave_at[BM_JOIN / 64];
   int* s_open = (int*)(s_at + cap);                                 // [threads, at least 192] stretches to go through
-  __shared__ int s_n, s_left;
+  __shared__ int s_n, s_left, s_left_out, s_greater;
+  __shared__ uint64_t s_edge;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, waves = threads >> 6;
   const int K = a.c.K, W = a.c.W, C = a.stretches, keep = a.keep;
@@ -393,7 +419,7 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
   const int n0 = tid < total ? stat[tid].n : 0;
   const int n_first = total <= 64 && lane < total ? stat[lane].n : 0;
   const BmPow pow(lane);
-  if (tid == 0) { s_n = 0; s_left = 0; }
+  if (tid == 0) { s_n = 0; s_left = 0; s_left_out = 0; }
   // the lanes of a beam: a power of two
   int g = 1;
   while (g < C && g < 64) g *= 2;
@@ -414,12 +440,12 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
         const BmStat s = st[c];
         if (s.sum != s.sum) sum = s.sum;             // (NaN stays)
         if (!(s.top > -__builtin_inff())) continue;  // nothing allowed there
-        if (s.ref == 0.0) {
+        if (s.ref == 0.0f) {
           top = fmaxf(top, s.top);
           sum += s.sum;
         } else {
-          const double m = fmax(ref, s.ref);
-          far = far * exp(ref - m) + s.sum * exp(s.ref - m);
+          const double m = fmax(ref, (double)s.ref);
+          far = far * exp(ref - m) + s.sum * exp((double)s.ref - m);
           ref = m;
         }
       }
@@ -454,6 +480,23 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
   auto key_of = [&](float x, int g) {   // (in this order: where x is the whole normaliser, the score stays what it was)
     const uint32_t k = cs_div(g, a.by_stretches);
     return bm_key64(s_before[k] + ((double)x - s_lse[k]));
+  };
+  // The best score that stretch g may have left out, 0 for none.  Within a beam it is no better than W kept ones, and it counts only
+  // where it is no worse than the worst of these: where one score has logits on both sides of the bound.
+  auto left_out = [&](int g) -> uint64_t {
+    const float cut = stat[g].cut;
+    if (cut == BM_LOWEST) return 0;
+    if (cut == cut) {   // (the float32 before it; both zeros are one)
+      const uint64_t at = key_of(cut, g);
+      return key_of(cut == 0.0f ? -1.401298464e-45f : bm_value(bm_key(cut) - 1), g) == at ? at : 0;
+    }
+    const float* x = item_x + (int64_t)g * keep;        // (the larger ones come first)
+    const int n = stat[g].n;
+    const float last = x[n - 1];
+    const uint64_t at = key_of(last, g);
+    bool one = x[n] > -__builtin_inff() && key_of(x[n], g) == at;
+    for (int r = 0; !one && x[r] > last; ++r) one = key_of(x[r], g) == at;
+    return one ? at : 0;
   };
   // a bound from below; none where there are few candidates
   uint64_t t = 1;
@@ -507,6 +550,7 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
     }
     t = t32 > 1 ? (uint64_t)t32 << 32 : 1;
   }
+  uint64_t below = 0;                  // the best score that this thread's stretches may have left out
   // stretches whose largest logit reaches the bound are gone through by 16 lanes each
   for (int g0 = 0; g0 < total; g0 += threads) {
     __syncthreads();
@@ -515,7 +559,11 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
     const int g = g0 + tid;
     if (g < total) {
       const float x = g0 == 0 ? top0 : stat[g].top;
-      if (x > -__builtin_inff() && key_of(x, g) >= t) s_open[atomicAdd(&s_left, 1)] = g;
+      if (x > -__builtin_inff() && key_of(x, g) >= t) {
+        s_open[atomicAdd(&s_left, 1)] = g;
+        const uint64_t u = left_out(g);
+        if (u >= t) { below = u > below ? u : below; s_left_out = 1; }
+      }
     }
     __syncthreads();
     const int open = s_left;
@@ -540,6 +588,8 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
     a.tokens[o] = key ? at & 0xffffffff : -1;
   };
   const int n = s_n;
+  uint64_t edge = 0;                   // the W-th best score, and how many results are better
+  int greater = 0;
   if (n <= cap) {
     // ranks by counting: each candidate against all.  Where there are many (W above 32), those from a bound on that W to 32
     // more reach, bisected
@@ -598,40 +648,99 @@ __device__ __forceinline__ void bm_join(const BmArgs& a, int64_t b, const BmStat
         before += other > key;
         equal += other == key;
       }
+      const int more = before;
       if (equal > 1 && before < W)
         for (int j = 0; j < m; ++j) before += s_key[j] == key && s_at[j] < at;
       if (before < W) put(before, key, at);
+      if (before == W - 1) { s_edge = key; s_greater = more; }
     }
     for (int w = n + tid; w < W; w += threads) put(w, 0, 0);
-    return;
+    if (n < W || !s_left_out) return;
+    __syncthreads();
+    edge = s_edge;
+    if (below >= edge) s_left_out = 2;
+    __syncthreads();
+    if (s_left_out != 2) return;
+    greater = s_greater;
   }
   // many equal scores: the results one by one, each the best of what comes after the one before
-  uint64_t last = ~0ull;
-  int64_t last_at = -1;
-  for (int w = 0; w < W; ++w) {
-    uint64_t key = 0;
-    int64_t at = 0;
-    for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {
-      const int g = cs_div(i, a.by_keep);
-      if ((int)i - g * keep >= stat[g].n) continue;
-      const uint64_t u = key_of(item_x[i], g);
-      const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item_v[i];
-      if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
+  for (;;) {
+    if (edge) {
+      // Stretches that may have left out some of the W-th best score get lists that are whole: of what they kept the better ones, and
+      // then the first values of that score.  A wavefront per stretch.
+      auto ahead = [](uint64_t m) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)); };
+      const BmArgs& args = bm_args();
+      const int want = W - greater;                // (in all; with the better ones of a stretch no more than W)
+      for (int g = wave; g < total; g += waves) {
+        if (!(stat[g].top > -__builtin_inff()) || left_out(g) < edge) continue;
+        const int n = stat[g].n;
+        float* gx = item_x + (int64_t)g * keep;
+        int32_t* gv = item_v + (int64_t)g * keep;
+        int c = 0;
+        for (int r0 = 0; r0 < n; r0 += 64) {       // (to places that have been read: the stores wait for the loads)
+          const bool there = r0 + lane < n;
+          const float x = there ? gx[r0 + lane] : 0.0f;
+          const int32_t v = there ? gv[r0 + lane] : 0;
+          const bool better = there && key_of(x, g) > edge;
+          const uint64_t m = __ballot(better);
+          if (better) { gx[c + ahead(m)] = x; gv[c + ahead(m)] = v; }
+          c += __popcll(m);
+        }
+        const int k = (int)cs_div(g, a.by_stretches);
+        const int64_t at = b * args.c.logits_stride[0] + k * args.c.logits_stride[1], mask_at = b * args.c.mask_stride[0] + k * args.c.mask_stride[1];
+        const int64_t v1 = (int64_t)(g - k * C + 1) * args.len, end = v1 < args.c.V ? v1 : args.c.V;
+        int found = 0;
+        for (int64_t v0 = v1 - args.len; v0 < end && found < want; v0 += 64) {
+          const int64_t v = v0 + lane;
+          float x = -__builtin_inff();
+          if (v < end && !(args.mask && !args.mask[mask_at + v])) {
+            if (args.c.logits_type == CS_TYPE_F32) x = ((const float*)args.logits)[at + v];
+            else if (args.c.logits_type == CS_TYPE_BF16) x = __uint_as_float((uint32_t)((const uint16_t*)args.logits)[at + v] << 16);
+            else x = (float)((const _Float16*)args.logits)[at + v];
+          }
+          const bool mine = x > -__builtin_inff() && key_of(x, g) == edge;
+          const uint64_t m = __ballot(mine);
+          const int place = c + found + ahead(m);
+          if (mine && place < c + want) { gx[place] = x; gv[place] = (int32_t)v; }
+          found += __popcll(m);
+        }
+        if (lane == 0) stat[g].n = c + (found < want ? found : want);
+      }
+      __syncthreads();
     }
-    for (int o = 32; o; o >>= 1) {
-      const uint64_t u = __shfl_xor((unsigned long long)key, o);
-      const int64_t f = __shfl_xor((long long)at, o);
-      if (u > key || (u == key && f < at)) { key = u; at = f; }
+    uint64_t last = ~0ull;
+    int64_t last_at = -1;
+    for (int w = 0; w < W; ++w) {
+      uint64_t key = 0;
+      int64_t at = 0;
+      for (uint32_t i = tid; i < (uint32_t)(total * keep); i += threads) {
+        const int g = cs_div(i, a.by_keep);
+        if ((int)i - g * keep >= stat[g].n) continue;
+        const uint64_t u = key_of(item_x[i], g);
+        const int64_t f = (int64_t)cs_div(g, a.by_stretches) << 32 | item_v[i];
+        if ((u < last || (u == last && f > last_at)) && (u > key || (u == key && key && f < at))) { key = u; at = f; }
+      }
+      for (int o = 32; o; o >>= 1) {
+        const uint64_t u = __shfl_xor((unsigned long long)key, o);
+        const int64_t f = __shfl_xor((long long)at, o);
+        if (u > key || (u == key && f < at)) { key = u; at = f; }
+      }
+      __syncthreads();
+      if (lane == 0) { s_wave[wave] = key; s_wave_at[wave] = at; }
+      __syncthreads();
+      key = s_wave[0]; at = s_wave_at[0];
+      for (int v = 1; v < waves; ++v)
+        if (s_wave[v] > key || (s_wave[v] == key && s_wave_at[v] < at)) { key = s_wave[v]; at = s_wave_at[v]; }
+      if (tid == 0) put(w, key, at);
+      if (key != last) greater = w;
+      last = key;
+      last_at = key ? at : INT64_MAX;
     }
+    if (edge || !last) return;
+    edge = last;
+    if (below >= edge) s_left_out = 2;
     __syncthreads();
-    if (lane == 0) { s_wave[wave] = key; s_wave_at[wave] = at; }
-    __syncthreads();
-    key = s_wave[0]; at = s_wave_at[0];
-    for (int v = 1; v < waves; ++v)
-      if (s_wave[v] > key || (s_wave[v] == key && s_wave_at[v] < at)) { key = s_wave[v]; at = s_wave_at[v]; }
-    if (tid == 0) put(w, key, at);
-    last = key;
-    last_at = key ? at : INT64_MAX;
+    if (s_left_out != 2) return;
   }
 }
 
@@ -639,7 +748,7 @@ __global__ void __launch_bounds__(BM_JOIN) cs_beam_join_kernel(const BmArgs a, i
   extern __shared__ __align__(16) char lds[];
   const int64_t b = cs_block(), total = (int64_t)a.c.K * a.stretches;
   if (b >= a.c.B) return;
-  bm_join(a, b, a.stat + b * total, a.item_x + b * total * a.keep, a.item_v + b * total * a.keep, lds, cap);
+  bm_join(b, a.stat + b * total, a.item_x + b * total * a.keep, a.item_v + b * total * a.keep, lds, cap);
 }
 
 // Both in one launch, where an example has few stretches: a wavefront each, which leave what they keep in LDS.  Saves a launch (512 x
@@ -657,7 +766,7 @@ __global__ void __launch_bounds__(BM_ONE * 64) cs_beam_one_kernel(const BmArgs a
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = cs_div(w, a.by_stretches);
   bm_scan<T, MASK, LANE>(a, (uint32_t)b * a.c.K + k, w - k * a.stretches, stat + w, item_x + w * keep, item_v + w * keep);
   __syncthreads();
-  bm_join(a, b, stat, item_x, item_v, lds + total * (sizeof(BmStat) + keep * 8), cap);
+  bm_join(b, stat, item_x, item_v, lds + total * (sizeof(BmStat) + keep * 8), cap);
 }
 
 // values per lane of a stretch: 32 where that fills the chip (6 wavefronts on each of its 1024 SIMDs), else, or where fewer hold
@@ -728,6 +837,7 @@ extern "C" int cs_beam_select(const cs_beam_cfg* c, const void* scores, const vo
   a.scores = scores; a.logits = logits; a.mask = mask; a.finished = finished;
   a.stretches = stretches_of(*c);
   a.keep = keep_of(*c);
+  a.len = 64 * lane_values(*c);
   const int64_t items = (int64_t)c->B * c->K * a.stretches;
   a.stat = (BmStat*)workspace;
   a.item_x = (float*)(a.stat + items);

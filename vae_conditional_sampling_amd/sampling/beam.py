@@ -51,11 +51,12 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
     first step of a search starts from one beam).  ``logits`` [B,K,V] float32 / bfloat16 / float16, the values adjacent in
     memory, any strides of the other axes.  A continuation scores
     ``scores + (logits - logsumexp(logits))``, or ``scores + logits`` with ``normalise=False``, formed in 64 bits;
-    equal scores go to the lowest (beam, value).  ``mask`` (bool, broadcastable to [B,K,V]; True = allowed): what is not
-    allowed takes no part in the normaliser either and may hold anything.  ``finished`` [B,K] (bool): such a beam only
-    continues with ``end_token``, at its score; its logits are not read.  NaN and -inf are never chosen; a beam with a NaN or
-    +inf among its allowed logits has no continuations (``normalise``).  An example with fewer than ``width`` continuations
-    ends in score -inf, token -1 and the slot's own index as parent."""
+    equal scores go to the lowest (beam, value), also where 64 bits do not tell different logits apart (a beam at -1e30).
+    ``mask`` (bool, broadcastable to [B,K,V]; True = allowed): what is not allowed takes no part in the normaliser either and
+    may hold anything.  ``finished`` [B,K] (bool): such a beam only continues with ``end_token``, at its score; its logits are
+    not read.  NaN and -inf are never chosen; a beam with a NaN or +inf among its allowed logits has no continuations
+    (``normalise``).  An example with fewer than ``width`` continuations ends in score -inf, token -1 and the slot's own index
+    as parent."""
     if logits.dim() != 3:
         raise _lib.CsError(f"logits must be [B,K,V], got {tuple(logits.shape)}")
     B, K, V = logits.shape
