@@ -515,7 +515,7 @@ int cs_beam_select(const cs_beam_cfg* cfg, const void* scores, const void* logit
 /* dst[o,b,w,:] = src[o,b,parents[b,w],:] for o < outer, b < B, w < W; rows of row_bytes adjacent bytes, the strides of
  * (outer, example, chain) in bytes.  A parent outside [0,K) leaves its row of dst as it was.  In place with
  * src == dst: W == K <= 64 and equal strides; otherwise the memory from the first to the last byte of either must not
- * overlap.  Rows of dst must not overlap each other. */
+ * overlap.  Rows of dst must not overlap each other, and parents must not lie among them. */
 int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_t B, int32_t K, int32_t W, int64_t row_bytes,
                     const int64_t src_stride[3], const int64_t dst_stride[3], const int64_t* parents, void* stream);
 

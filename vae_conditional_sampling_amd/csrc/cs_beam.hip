@@ -1074,6 +1074,8 @@ extern "C" int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_
       CS_REQUIRE(dst_stride[order[i]] >= dst_end, "rows of the destination overlap");
       dst_end += (n_dst[order[i]] - 1) * dst_stride[order[i]];
     }
+  const char* after = (const char*)(parents + B * W);   // (threads that write rows would do so while others still read their parents)
+  CS_REQUIRE(after <= (const char*)dst || (const char*)dst + dst_end <= (const char*)parents, "parents lie in the destination");
   if (in_place) {
     CS_REQUIRE(W == K && K <= 64, "in place: as many chains as before, at most 64");
     for (int i = 0; i < 3; ++i) CS_REQUIRE(n_src[i] == 1 || src_stride[i] == dst_stride[i], "in place: one layout");

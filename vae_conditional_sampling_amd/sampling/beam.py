@@ -111,8 +111,9 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
 
 @functools.lru_cache(maxsize=256)
 def _rows(shape, strides, size, axis):
-    """(outer, strides in bytes of (outer, example, chain), bytes of a row) of a tensor [outer..., B, K, row...], or None if
-    the outer axes do not collapse into one stride or a row is not adjacent in memory."""
+    """(outer, strides in bytes of (outer, example, chain), bytes of a row, bytes from the first row's start to the last one's
+    end) of a tensor [outer..., B, K, row...], or None if the outer axes do not collapse into one stride or a row is not
+    adjacent in memory."""
     row = 1
     for n, s in zip(reversed(shape[axis + 2:]), reversed(strides[axis + 2:])):
         if n != 1 and s != row:
@@ -127,7 +128,8 @@ def _rows(shape, strides, size, axis):
         elif s != stride * outer:
             return None
         outer *= n
-    return outer, (C.c_int64 * 3)(stride * size, strides[axis] * size, strides[axis + 1] * size), row * size
+    end = (outer - 1) * stride + (shape[axis] - 1) * strides[axis] + (shape[axis + 1] - 1) * strides[axis + 1] + row
+    return outer, (C.c_int64 * 3)(stride * size, strides[axis] * size, strides[axis + 1] * size), row * size, end * size
 
 
 def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: int = 0,
@@ -138,7 +140,7 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: in
     ``parents`` [B,W] int64; a parent outside [0,K) leaves its row of ``out`` as it was.  ``out=None`` returns a new tensor (a
     row without a parent is zero there); ``out=states`` works in place (W = K <= 64): rows that keep their place are not
     touched, so a search that leaves survivors where they are moves only what changed.  ``out`` elsewhere must not overlap
-    ``states``."""
+    ``states``.  ``parents`` may be a part of ``out`` (a history of parents that is reordered itself): it is copied first."""
     if batch_dim < 0:
         batch_dim += states.dim()
     if not 0 <= batch_dim <= states.dim() - 2:
@@ -167,6 +169,9 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: in
         states = states.contiguous()
         src = _rows(shape, states.stride(), size, batch_dim)
     parents = parents.contiguous()
-    _lib.call_on(dev, _lib.lib().cs_beam_reorder, states.data_ptr(), out.data_ptr(), src[0], B, K, W, src[2], src[1], dst[1],
-                 parents.data_ptr())
+    to, parents_at = out.data_ptr(), parents.data_ptr()
+    if parents_at < to + dst[3] and to < parents_at + 8 * B * W:   # parents that are a part of what is written
+        parents = parents.clone()
+        parents_at = parents.data_ptr()
+    _lib.call_on(dev, _lib.lib().cs_beam_reorder, states.data_ptr(), to, src[0], B, K, W, src[2], src[1], dst[1], parents_at)
     return out
