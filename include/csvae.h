@@ -539,12 +539,12 @@ int64_t cs_qcache_record_bytes(int32_t fmt, int32_t group, int32_t D);   /* -1: 
 /* Quantises X[n,B,K,D] (n <= T; D values adjacent, the strides of (step, example, chain) in elements) into the slots
  * (start + i) mod T, i < n.  start[B,K] (NULL: start0 for all; negative: nothing of that chain is written),
  * count[B,K] (NULL: n): only the first count states of a chain are read and written; every other record stays as it
- * is. */
+ * is.  X must not lie in the ring. */
 int cs_qcache_write(const cs_qcache* c, const void* X, int32_t x_type, int64_t n, const int64_t x_stride[3],
                     const int64_t* start, int64_t start0, const int64_t* count, void* stream);
 /* out[i,b,j,:] = the state at slot slots[i,b,j] (NULL: (start0 + i) mod T) of chain chains[i,b,j] (NULL: j, and J must
  * be K) of example b; zeros where slot or chain do not exist.  slots / chains: int64 [N,B,J]; out_stride of
- * (i, example, j) in elements; rows of out must not overlap.  A value beyond the largest finite one of out_type reads as that
+ * (i, example, j) in elements; rows of out must not overlap each other nor what is read.  A value beyond the largest finite one of out_type reads as that
  * one: a finite state never reads as an infinity. */
 int cs_qcache_read(const cs_qcache* c, const int64_t* slots, int64_t start0, const int64_t* chains, int64_t N, int32_t J,
                    void* out, int32_t out_type, const int64_t out_stride[3], void* stream);

@@ -1058,22 +1058,14 @@ extern "C" int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_
   if (outer == 0 || B == 0 || row_bytes == 0) return CS_OK;
   CS_REQUIRE(src && dst && src_stride && dst_stride && parents, "null argument");
   const bool in_place = src == dst;
-  int64_t src_end = row_bytes, dst_end = row_bytes;
+  int64_t src_end = row_bytes;
   const int64_t n_src[3] = {outer, B, K}, n_dst[3] = {outer, B, W};
   for (int i = 0; i < 3; ++i) {
     CS_REQUIRE(src_stride[i] >= 0 && dst_stride[i] >= 0, "negative stride");
     src_end += (n_src[i] - 1) * src_stride[i];
   }
-  // the destination's rows must not meet: from the closest axis on, every stride clears what lies within
-  int order[3] = {0, 1, 2};
-  for (int i = 0; i < 2; ++i)
-    for (int j = 0; j < 2; ++j)
-      if (dst_stride[order[j]] > dst_stride[order[j + 1]]) { const int t = order[j]; order[j] = order[j + 1]; order[j + 1] = t; }
-  for (int i = 0; i < 3; ++i)
-    if (n_dst[order[i]] > 1) {
-      CS_REQUIRE(dst_stride[order[i]] >= dst_end, "rows of the destination overlap");
-      dst_end += (n_dst[order[i]] - 1) * dst_stride[order[i]];
-    }
+  const int64_t dst_end = cs_rows_apart(n_dst, dst_stride, row_bytes);
+  CS_REQUIRE(dst_end >= 0, "rows of the destination overlap");
   const char* after = (const char*)(parents + B * W);   // (threads that write rows would do so while others still read their parents)
   CS_REQUIRE(after <= (const char*)dst || (const char*)dst + dst_end <= (const char*)parents, "parents lie in the destination");
   if (in_place) {

@@ -26,3 +26,20 @@ inline dim3 cs_grid(int64_t blocks) {
   return blocks <= ROW ? dim3((unsigned)blocks) : dim3((unsigned)ROW, (unsigned)((blocks + ROW - 1) >> CS_GRID_SHIFT));
 }
 __device__ __forceinline__ uint32_t cs_block() { return (blockIdx.y << CS_GRID_SHIFT) + blockIdx.x; }
+
+// Rows of `row` units along three axes: the units from the first one's start to the last one's end, or -1 where rows may meet (from
+// the closest axis on, every stride has to clear what lies within).
+inline int64_t cs_rows_apart(const int64_t n[3], const int64_t stride[3], int64_t row) {
+  int order[3] = {0, 1, 2};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
+      if (stride[order[j]] > stride[order[j + 1]]) { const int t = order[j]; order[j] = order[j + 1]; order[j + 1] = t; }
+  int64_t end = row;
+  for (int i = 0; i < 3; ++i) {
+    const int a = order[i];
+    if (n[a] <= 1) continue;
+    if (stride[a] < end) return -1;
+    end += (n[a] - 1) * stride[a];
+  }
+  return end;
+}

@@ -371,6 +371,10 @@ void launch_type(const QcArgs& a, int type, int R, bool packed, dim3 grid, hipSt
   else launch_rows<WRITE, FMT, _Float16>(a, R, packed, grid, st);
 }
 
+bool apart(const void* p, int64_t p_bytes, const void* q, int64_t q_bytes) {
+  return !p || !q || (const char*)p + p_bytes <= (const char*)q || (const char*)q + q_bytes <= (const char*)p;
+}
+
 // n steps of B * inner rows
 template <bool WRITE>
 int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStream_t st) {
@@ -385,6 +389,21 @@ int launch(QcArgs& a, int64_t n, int32_t inner, int64_t start0, int type, hipStr
   CS_REQUIRE(((uintptr_t)c.data & 15) == 0, "the ring must be 16-byte aligned");
   a.record = cs_qcache_record_bytes(c.fmt, c.group, c.D);
   a.code_bytes = (int32_t)code_bytes_of(c.fmt, c.D);
+  // what is written is neither written twice nor read by other threads
+  const int64_t sizes[3] = {n, c.B, inner}, size = type == CS_TYPE_F32 ? 4 : 2;
+  const int64_t ring = c.T * c.B * c.K * a.record, indices = (int64_t)a.rows * 8;
+  int64_t end = c.D;
+  for (int i = 0; i < 3; ++i) {
+    CS_REQUIRE(a.stride[i] >= 0, "negative stride");
+    end += (sizes[i] - 1) * a.stride[i];
+  }
+  if (WRITE) {
+    CS_REQUIRE(apart(a.x, end * size, c.data, ring), "states lie in the ring");
+  } else {
+    CS_REQUIRE(cs_rows_apart(sizes, a.stride, c.D) >= 0, "rows of the output overlap");
+    CS_REQUIRE(apart(a.out, end * size, c.data, ring) && apart(a.out, end * size, a.slots, indices) &&
+               apart(a.out, end * size, a.from, indices), "the output lies in what is read");
+  }
   if (WRITE)
     while (a.c.group > QC_LANE && c.D <= a.c.group / 2) a.c.group /= 2;   // (a row of one group, cut to what it holds)
   a.lanes = WRITE ? (c.D + a.c.group - 1) / a.c.group * (a.c.group / QC_LANE) : (c.D + QC_LANE - 1) / QC_LANE;
