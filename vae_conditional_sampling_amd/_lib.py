@@ -169,6 +169,8 @@ class cs_qcache(C.Structure):
                 ("fmt", C.c_int32), ("group", C.c_int32)]
 
 
+INT32_MAX = 0x7fffffff   # (ctypes cuts larger integers without a word)
+
 # element types and formats of the beam / quantised-history entry points
 CS_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 CS_QFMT = {"int8": 0, "mxfp8": 1, "mxfp4": 2}

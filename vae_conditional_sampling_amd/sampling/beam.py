@@ -34,6 +34,8 @@ def _flags(t, what):
 @functools.lru_cache(maxsize=256)
 def _select_cfg(B, K, V, width, logits_type, scores_type, normalise, end_token, ls0, ls1, ms0, ms1):
     """(cs_beam_cfg, bytes of workspace) of calls of one shape; read only."""
+    if max(B, K, V, end_token) > _lib.INT32_MAX or end_token < 0:   # (they would wrap)
+        raise _lib.CsError(f"at most 2^31 - 1 examples, beams and values and an end token among these, got {B}, {K}, {V}, {end_token}")
     pair = C.c_int64 * 2
     cfg = _lib.cs_beam_cfg(B, K, V, width, logits_type, scores_type, normalise, end_token, pair(ls0, ls1), pair(ms0, ms1))
     nbytes = _lib.lib().cs_beam_select_workspace(C.byref(cfg))
@@ -114,6 +116,8 @@ def _rows(shape, strides, size, axis):
     """(outer, strides in bytes of (outer, example, chain), bytes of a row, bytes from the first row's start to the last one's
     end) of a tensor [outer..., B, K, row...], or None if the outer axes do not collapse into one stride or a row is not
     adjacent in memory."""
+    if max(shape[axis:axis + 2]) > _lib.INT32_MAX:
+        raise _lib.CsError(f"at most 2^31 - 1 examples and chains, got {list(shape[axis:axis + 2])}")
     row = 1
     for n, s in zip(reversed(shape[axis + 2:]), reversed(strides[axis + 2:])):
         if n != 1 and s != row:

@@ -207,6 +207,8 @@ class QuantisedHistory:
         group = (64 if fmt == "int8" else 32) if group is None else int(group)
         self.max_history_length, self.batch_shape, self.fmt, self.group = int(max_history_length), tuple(batch_shape), fmt, group
         B, K, D = self.batch_shape
+        if max(self.max_history_length, B, K, D, abs(group)) > _lib.INT32_MAX:
+            raise _lib.CsError(f"no history of {self.max_history_length} states {self.batch_shape}: at most 2^31 - 1 of each")
         self.record_bytes = int(_lib.lib().cs_qcache_record_bytes(_lib.CS_QFMT[fmt], group, D))
         if self.record_bytes < 0 or self.max_history_length < 1 or K < 1:
             raise _lib.CsError(f"no history of {self.max_history_length} states {self.batch_shape} as {fmt}, groups of {group}")
@@ -230,6 +232,10 @@ class QuantisedHistory:
             raise _lib.CsError(f"{what} must be int64 {list(shape)}, got {t.dtype} {list(t.shape)}")
         return t.contiguous()
 
+    def _slot(self, start):
+        start = int(start)
+        return start % self.max_history_length if start >= 0 else -1   # (which the library refuses)
+
     def write(self, X, start, counts=None):
         """Quantise ``X`` [n,B,K,D] or [B,K,D] (float32 / bfloat16 / float16, any strides with D adjacent; n <= T) into the
         slots ``start .. start + n - 1`` (mod T).  ``start``: an int, or an int64 tensor [B,K] with a position per chain (negative:
@@ -247,7 +253,7 @@ class QuantisedHistory:
             start = self._int64(start, (B, K), "start")
             start_at = start.data_ptr()
         else:
-            first = int(start)
+            first = self._slot(start)
         if counts is not None:
             counts = self._int64(counts, (B, K), "counts")
             counts_at = counts.data_ptr()
@@ -266,7 +272,8 @@ class QuantisedHistory:
         infinity)."""
         B, K, D = self.batch_shape
         shape = tuple(slots.shape)
-        if len(shape) not in (2, 3) or shape[-2] != B or slots.dtype != torch.int64 or (chains is None and shape[-1] != K):
+        if len(shape) not in (2, 3) or shape[-2] != B or slots.dtype != torch.int64 or (chains is None and shape[-1] != K) \
+                or shape[-1] > _lib.INT32_MAX:
             raise _lib.CsError(f"slots must be int64 [N,{B},{K}] (or [N,{B},J] with chains), got {slots.dtype} {list(shape)}")
         chains_at = None
         if chains is not None:
@@ -287,7 +294,7 @@ class QuantisedHistory:
         out, kind, strides = self._out(out, (int(n), B, K, D), dtype)
         if out.numel():
             dev = _lib.on_device(self._data, out)
-            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring, None, int(start), None, int(n), K, out.data_ptr(), kind,
+            _lib.call_on(dev, _lib.lib().cs_qcache_read, self._ring, None, self._slot(start), None, int(n), K, out.data_ptr(), kind,
                          _STRIDES(*strides[:3]))
         return out
 
@@ -310,5 +317,7 @@ class QuantisedHistory:
         """The records of every chain follow ``parents`` [B,K] in place (``beam.reorder_states``: K <= 64), in the first ``steps``
         slots (None: all)."""
         from .beam import reorder_states
+        if steps is not None and int(steps) < 0:
+            raise _lib.CsError(f"negative number of steps {steps}")
         data = self._data if steps is None else self._data[:int(steps)]
         reorder_states(data, parents, batch_dim=1, out=data)
