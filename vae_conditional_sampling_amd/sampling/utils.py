@@ -212,9 +212,21 @@ class QuantisedHistory:
         self.record_bytes = int(_lib.lib().cs_qcache_record_bytes(_lib.CS_QFMT[fmt], group, D))
         if self.record_bytes < 0 or self.max_history_length < 1 or K < 1:
             raise _lib.CsError(f"no history of {self.max_history_length} states {self.batch_shape} as {fmt}, groups of {group}")
-        self._desc = _lib.cs_qcache(None, self.max_history_length, B, K, D, _lib.CS_QFMT[fmt], group)
-        self._ring = C.byref(self._desc)
+        self._describe()
         self.data = torch.zeros((self.max_history_length, B, K, self.record_bytes), dtype=torch.uint8, device=device)
+
+    def _describe(self):
+        self._desc = _lib.cs_qcache(None, self.max_history_length, *self.batch_shape, _lib.CS_QFMT[self.fmt], self.group)
+        self._ring = C.byref(self._desc)
+
+    # (a copy, shallow or deep, has a descriptor of its own: it names the memory of that copy's ``data``)
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_desc", "_ring")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._describe()
+        self.data = self._data
 
     @property
     def data(self):
