@@ -7,7 +7,7 @@ import pickle
 import pytest
 import torch
 
-from vae_conditional_sampling_amd.sampling.utils import QuantisedHistory
+from vae_conditional_sampling_amd.sampling.utils import ImputationHistoryQueue, QuantisedHistory
 
 
 def given(q):
@@ -25,6 +25,31 @@ def test_a_copy_has_a_ring_of_its_own():
     for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
         assert torch.equal(other.data, q.data) and given(other) == other.data.data_ptr() != own
         assert (other.fmt, other.group, other.record_bytes, other._desc.D) == ("int8", 32, q.record_bytes, 7)
+
+
+@pytest.mark.parametrize("storage", [None, "mxfp4"])
+def test_a_queue_uses_the_ring_it_is_given(storage):
+    q = ImputationHistoryQueue(4, (2, 3, 7), device="cpu", storage=storage)
+    ring = q.history_queue.clone()
+    q.history_queue = ring
+    assert q.history_queue is ring
+    if storage:
+        assert given(q.quantised) == ring.data_ptr()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("storage", [None, "int8", "mxfp8", "mxfp4"])
+def test_a_queue_goes_on_with_a_restored_ring(storage):
+    g = torch.Generator().manual_seed(2)
+    X = [torch.randn(2, 3, 43, generator=g).cuda() for _ in range(4)]
+    q, other = (ImputationHistoryQueue(4, (2, 3, 43), storage=storage) for _ in range(2))
+    for x in X[:3]:
+        q.enqueue_batch(x)
+    other.history_queue, other.tail_idx, other.full = q.history_queue.clone(), q.tail_idx, q.full
+    for queue in (q, other):
+        queue.enqueue_batch(X[3])
+    a, b = (queue.concat_history(X[0], [0, 2, 3], chain_of_proposal=[1, 0, 2]) for queue in (q, other))
+    assert torch.equal(a, b) and bool(a[:, 3:].any())
 
 
 @pytest.mark.gpu

@@ -38,11 +38,22 @@ class ImputationHistoryQueue(object):
         self.quantised = None
         if storage is not None:
             self.quantised = QuantisedHistory(self.max_history_length, self.batch_shape, storage, device=device)
-            self.history_queue = self.quantised.data
             self._chain_ids = None
             return
         self.history_queue = torch.empty((self.max_history_length, B, K, D),
                                          dtype=torch.uint8 if self.u8 else torch.float32, device=device)
+
+    @property
+    def history_queue(self):
+        """The ring [T,B,K,D], with ``storage`` its records; may be replaced by one of the same shape."""
+        return self._history_queue if self.quantised is None else self.quantised.data
+
+    @history_queue.setter
+    def history_queue(self, ring):
+        if self.quantised is None:
+            self._history_queue = ring
+        else:
+            self.quantised.data = ring
 
     def __len__(self):
         assert self.tail_idx > -1, 'Queue is empty.'
