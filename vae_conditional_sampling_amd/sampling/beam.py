@@ -81,7 +81,10 @@ def beam_select(scores: Optional[torch.Tensor], logits: torch.Tensor, width: int
         ls = logits.stride()
     ms = (0, 0)
     if mask is not None:
-        mask = _flags(mask, "mask").expand(B, K, V)
+        mask = _flags(mask, "mask")
+        if mask.dim() > 3 or any(n not in (1, m) for n, m in zip(reversed(mask.shape), (V, K, B))):
+            raise _lib.CsError(f"mask must broadcast to [{B},{K},{V}], got {list(mask.shape)}")
+        mask = mask.expand(B, K, V)
         if mask.stride(2) != 1 and V > 1:
             mask = mask.contiguous()
         ms = mask.stride()
