@@ -163,18 +163,14 @@ __device__ __forceinline__ void qc_decode(const uint32_t* codes, uint32_t scale,
              c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[0], 1.0f, 3);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
   }
-  // elements end at 1.75 * 2^8 and 1.5 * 2^2: no scale up to this one leaves the range
-  constexpr int SAFE = QcMost<T>::e - (FMT == CS_QFMT_MXFP8 ? 8 : 2);
-  if (__ballot(e > SAFE)) {
-#pragma unroll
-    for (int i = 0; i < QC_LANE; ++i) {   // (a NaN stays: fmax and fmin would pass it over)
-      const float p = __builtin_amdgcn_ldexpf(v[i], e);
-      v[i] = scale == 255u ? __builtin_nanf("") : __builtin_fabsf(p) > most ? __builtin_copysignf(most, p) : p;
-    }
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < QC_LANE; ++i) v[i] = __builtin_amdgcn_ldexpf(v[i], e);
+  // elements end at 1.75 * 2^8 and 1.5 * 2^2: no scale up to this one leaves the range
+  if (__builtin_expect(e > QcMost<T>::e - (FMT == CS_QFMT_MXFP8 ? 8 : 2), 0)) {
+#pragma unroll
+    for (int i = 0; i < QC_LANE; ++i)   // (a NaN stays: fmax and fmin would pass it over)
+      v[i] = scale == 255u ? __builtin_nanf("") : __builtin_fabsf(v[i]) > most ? __builtin_copysignf(most, v[i]) : v[i];
+  }
 }
 
 // the slot of step i of a chain of a call that runs from `start` on; -1: not in the call
