@@ -508,7 +508,8 @@ int64_t cs_beam_select_workspace(const cs_beam_cfg* cfg);
  * none.  out_scores[B,W], parents[B,W], tokens[B,W] (int64); where there are fewer than W candidates: -inf, the
  * slot's own index (at most K-1), -1.  Scores that 64 bits do not tell apart are equal, whatever their logits: they go to the
  * lowest k*V + v like all equal ones.
- * Two launches; the result does not depend on anything but the arguments. */
+ * One launch where an example has few stretches of values, else two; the result does not depend on anything but the
+ * arguments. */
 int cs_beam_select(const cs_beam_cfg* cfg, const void* scores, const void* logits, const uint8_t* mask,
                    const uint8_t* finished, void* out_scores, int64_t* parents, int64_t* tokens, void* workspace,
                    int64_t workspace_bytes, void* stream);
@@ -524,7 +525,8 @@ int cs_beam_reorder(const void* src, void* dst, int64_t outer, int64_t B, int32_
  * scales of its groups of `group` consecutive values.
  *   CS_QFMT_INT8   groups of 32, 64 or 128; scale s = max(float32(largest finite magnitude / 127), 2^-126); code = the
  *                  integer nearest to x / s, ties to even; -128 where x is not finite (reads as NaN)
- *   CS_QFMT_MXFP8  OCP Microscaling e4m3, groups of 32, scale 2^e with the smallest e >= -127 that clips nothing; nearest,
+ *   CS_QFMT_MXFP8  OCP Microscaling e4m3, groups of 32, scale 2^e with the smallest e >= -127 that clips nothing (OCP's own
+ *                  conversion clips the largest mantissas instead and has a bit more for the rest of such a group); nearest,
  *                  ties to even; not finite: NaN
  *   CS_QFMT_MXFP4  the same with e2m1; a group with a value that is not finite reads as NaN */
 #define CS_QFMT_INT8 0

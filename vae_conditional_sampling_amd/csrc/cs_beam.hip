@@ -175,9 +175,10 @@ __device__ __forceinline__ uint32_t bm_wave_threshold(uint32_t key, int W) {
   return t;
 }
 
-// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 618 of them for 2048 values, 364 of
-// these the 64-bit exponentials (91 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 82 to 90 us, 85 % of
-// them issuing, where their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB) take 37 us, 4.5 TB/s.
+// One wavefront per stretch.  Bound by vector instructions where the logits have 16 bits: 619 of them for 2048 values, 364 of
+// these the 64-bit exponentials (91 for 8 values of a lane); 64 x 16 rows of 131072 bfloat16 (268 MB) take 82 to 90 us, 81 % of the
+// launch's cycles issuing them, where their bytes alone would take 45.  In float32 it is bound by memory: 4096 rows of 10200 (167 MB)
+// take 33 to 38 us, 4.4 to 5.1 TB/s.  A value below -690 sends its stretch through the exponentials again: 103 -> 157 us with a third at -inf.
 // (Logits and values kept in two arrays, so that a kept one costs 4 instructions and not 8: 3 % faster.)
 // 32 values per lane measured 104 us there against 115 (16), 147 (8) and 164 (64: too few wavefronts fit); asking for the
 // next stretch before working on one (a fixed set of wavefronts) measured 141: twice the registers.
@@ -396,8 +397,9 @@ __global__ void __launch_bounds__(256, LANE == 32 && !MASK && BmElem<T>::N == 4 
   bm_scan<T, MASK, LANE>(a, row, item - row * a.stretches, a.stat + item, a.item_x + at, a.item_v + at);
 }
 
-// One workgroup per example; bound by its chain of dependent loads and barriers: 5.9 us for 4 beams of 32 stretches, 16 for 16 of
-// 64, 10 for 4096 examples of 5 stretches (W = 64: 34).
+// One workgroup per example; bound by its chain of dependent loads and barriers: 6.8 us for 4 beams of 32 stretches, 15 for 16 of
+// 64, 10 for 4096 examples of 5 stretches (W = 64: 46).  Lists that have to be completed cost the most where every beam's score swallows
+// its logits (all at -1e30): 4096 x 10200 in 75 us instead of 44, 64 x 16 x 131072 in 1.7 ms instead of 0.1.
 __device__ __forceinline__ void bm_join(int64_t b, BmStat* stat, float* item_x, int32_t* item_v, char* lds, int cap) {
   const BmArgs& a = bm_args();
   double* s_lse = (double*)lds;                                     // [K]

@@ -1,5 +1,6 @@
 // n / d for any 32-bit n by a multiplication (the round-up form of Granlund and Montgomery, 1994), d from 1 to 2^32 - 1: a
-// 64-bit division by a size of the call costs a lane several hundred instructions, a 32-bit one about forty.  And grids of more workgroups than a launch's first axis may hold.
+// 64-bit division by a size of the call costs a lane several hundred instructions, a 32-bit one about forty.  Also grids of more
+// workgroups than a launch's first axis may hold, and rows in memory that must not meet.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -18,8 +19,8 @@ __device__ __forceinline__ uint32_t cs_div(uint32_t n, const CsDiv& d) {   // (s
   return (t + ((n - t) >> d.s1)) >> d.s2;
 }
 
-// Workgroups of 256 to 1024 threads in two axes (an axis of a launch has to stay below 2^32 threads), and the number of one;
-// the last row may hold more workgroups than were asked for.  At most 2^36 of them.
+// Workgroups of up to 1024 threads in two axes (an axis of a launch has to stay below 2^32 threads), and the number of one;
+// the last row may hold up to 2^20 - 1 more workgroups than were asked for.  The number has 32 bits: callers stay at 2^31.
 constexpr int CS_GRID_SHIFT = 20;
 inline dim3 cs_grid(int64_t blocks) {
   constexpr int64_t ROW = 1ll << CS_GRID_SHIFT;

@@ -145,7 +145,7 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor, *, batch_dim: in
     ``batch_dim + 1`` are examples and chains: latents [B,K,Zd], a history [T,B,K,D] (``batch_dim=1``).
 
     ``parents`` [B,W] int64; a parent outside [0,K) leaves its row of ``out`` as it was.  ``out=None`` returns a new tensor (a
-    row without a parent is zero there); ``out=states`` works in place (W = K <= 64): rows that keep their place are not
+    row without a parent is zero there: all of it is filled first, half as many bytes again); ``out=states`` works in place (W = K <= 64): rows that keep their place are not
     touched, so a search that leaves survivors where they are moves only what changed.  ``out`` elsewhere must not overlap
     ``states``.  ``parents`` may be a part of ``out`` (a history of parents that is reordered itself): it is copied first."""
     if batch_dim < 0:

@@ -23,7 +23,9 @@ class ImputationHistoryQueue(object):
 
     ``storage`` (``int8`` | ``mxfp8`` | ``mxfp4``; no counterpart in the reference): the ring holds the imputations in 8 or 4
     bits (``QuantisedHistory``), for real-valued data whose float32 ring would not fit; slots and chains are drawn as for
-    the float32 ring, the historical proposals are what the ring reads back."""
+    the float32 ring, the historical proposals are what the ring reads back, observed values included.  ``concat_history`` uploads
+    its indices by copies that wait for the stream: an iteration of enqueueing and fetching takes 67 us instead of 17 at 512 examples
+    of 4 chains, 105 instead of 111 at 65536."""
 
     def __init__(self, max_history_length, batch_shape, dtype=torch.float32, device="cuda", storage=None):
         if dtype not in (torch.float32, torch.bool) or (storage is not None and dtype == torch.bool):
