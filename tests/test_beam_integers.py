@@ -19,10 +19,10 @@ def test_configurations():
 
 
 def test_layouts_and_rings():
-    for shape in ((1, FAR, 2, 3), (1, 2, FAR, 3)):
-        with pytest.raises(_lib.CsError, match="chains"):
-            beam._rows(shape, (0, 0, 0, 1), 4, 1)
-    assert beam._rows((FAR, 2, 2, 3), (12, 6, 3, 1), 4, 1)[0] == FAR       # (64 bits there)
+    with pytest.raises(_lib.CsError, match="chains"):
+        beam._rows((1, 2, FAR, 3), (0, 0, 0, 1), 4, 1)
+    assert beam._rows((FAR, 2, 2, 3), (12, 6, 3, 1), 4, 1)[0] == FAR       # (64 bits for the other axes)
+    assert beam._rows((2, FAR, 2, 3), (6 * FAR, 6, 3, 1), 4, 1)[3] == 4 * 12 * FAR
     for T, shape, group in ((FAR, (2, 3, 7), None), (4, (2, FAR, 7), None), (4, (2, 3, FAR), None), (4, (FAR, 3, 7), None),
                             (4, (2, 3, 7), (1 << 32) + 64)):
         with pytest.raises(_lib.CsError):

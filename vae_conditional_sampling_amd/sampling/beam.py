@@ -119,8 +119,8 @@ def _rows(shape, strides, size, axis):
     """(outer, strides in bytes of (outer, example, chain), bytes of a row, bytes from the first row's start to the last one's
     end) of a tensor [outer..., B, K, row...], or None if the outer axes do not collapse into one stride or a row is not
     adjacent in memory."""
-    if max(shape[axis:axis + 2]) > _lib.INT32_MAX:
-        raise _lib.CsError(f"at most 2^31 - 1 examples and chains, got {list(shape[axis:axis + 2])}")
+    if shape[axis + 1] > _lib.INT32_MAX:
+        raise _lib.CsError(f"at most 2^31 - 1 chains, got {shape[axis + 1]}")
     row = 1
     for n, s in zip(reversed(shape[axis + 2:]), reversed(strides[axis + 2:])):
         if n != 1 and s != row:
